@@ -33,8 +33,10 @@
 #include <algorithm>
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 #include "ecc_common.cuh"
+#include "paged.cuh"
 
 namespace ecc {
 
@@ -54,24 +56,6 @@ constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: fma(u, 8, kMagic + 96) rou
 constexpr int kCompressWarps = 8;
 constexpr int kVecPerWarp = 8;
 constexpr int kVecPerTile = kCompressWarps * kVecPerWarp;
-
-// Unsigned 32-bit division by a runtime constant d >= 1 (round-up method:
-// s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1, q = (umulhi(n,m) + n) >> s),
-// valid for every n < 2^32.
-struct FastDiv {
-    uint32_t d, m, s;
-};
-static inline FastDiv make_fastdiv(uint32_t d) {
-    FastDiv f;
-    f.d = d;
-    f.s = 0;
-    while ((1ull << f.s) < d) ++f.s;
-    f.m = (uint32_t)((((1ull << 32) * ((1ull << f.s) - d)) / d) + 1);
-    return f;
-}
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) {
-    return (uint32_t)(((uint64_t)__umulhi(n, f.m) + n) >> f.s);
-}
 
 struct __align__(16) QEntry {
     float thr;   // decision threshold inside this cell, +inf if none
@@ -261,6 +245,34 @@ struct CompressJobs {
     CompressJob j[2];
     int njobs;
 };
+// The same into pages: token l of sequence b goes to position pos[b] + l of
+// the page table when l < new_lens[b] (all L when null), and nowhere
+// otherwise; bs_b of the jobs is the stride of a page.  A position outside the
+// table, a page outside the pool or a count outside [0, L] writes nothing and
+// raises the flag of paged.cuh.
+struct PagedJobs : CompressJobs {
+    paged::PageTable t;
+    const int *pos, *new_lens;
+};
+__device__ __forceinline__ bool paged_dst(const PagedJobs &jobs, const CompressJob &jb, int b, int64_t h, int64_t l,
+                                          uint8_t *&dst) {
+    const int64_t L = jb.div_l.d;
+    if (jobs.new_lens) {
+        const int n = __ldg(jobs.new_lens + b);
+        if (n < 0 || n > L) atomicExch(&paged::g_paged_error, 5);
+        if (l >= n) return false;
+    }
+    const int64_t p = (int64_t)__ldg(jobs.pos + b) + l;
+    if (p < 0 || p >= jobs.t.capacity) {
+        atomicExch(&paged::g_paged_error, 5);
+        return false;
+    }
+    int slot;
+    const int page = jobs.t.page(b, (int)p, slot);
+    if (page < 0) return false;
+    dst = jb.blocks + ((int64_t)page * jb.bs_b + h * jb.bs_h + slot) * jb.rec;
+    return true;
+}
 
 // One warp's kVecPerWarp vectors of tile `tile`.  The fast pass (kExact =
 // false) gives up and returns false, before writing anything, when any of the
@@ -268,15 +280,18 @@ struct CompressJobs {
 // decision threshold, or a std near an fp32 rounding midpoint); the exact
 // pass handles those elements one by one.  Keeping the exact code out of the
 // fast pass keeps the hot loop small.
-template <bool kRotate, bool kExact>
+// (kGiven: the lane's block address and whether it has one come from the
+// caller instead of the strides.)
+template <bool kRotate, bool kExact, bool kGiven = false>
 __device__ __forceinline__ bool compress_warp(const __half *__restrict__ x, int64_t xs_b, int64_t xs_h, int64_t xs_l,
                                               uint8_t *__restrict__ blocks, int64_t bs_b, int64_t bs_h,
                                               FastDiv div_h, FastDiv div_l, uint32_t n_vec, uint32_t tile,
-                                              const QEntry *tab, uint32_t *st, uint32_t rec) {
+                                              const QEntry *tab, uint32_t *st, uint32_t rec,
+                                              uint8_t *given_dst = nullptr, bool given_valid = false) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane & 3, vsub = lane >> 2, base = lane & ~3;
     const uint32_t vi = tile * kVecPerTile + warp * kVecPerWarp + vsub;
-    const bool valid = vi < n_vec;
+    const bool valid = kGiven ? given_valid : vi < n_vec;
     const uint32_t row = fdiv(valid ? vi : 0u, div_l);
     const int64_t l = (valid ? vi : 0u) - row * div_l.d;
     const uint32_t bq = fdiv(row, div_h);
@@ -386,7 +401,7 @@ __device__ __forceinline__ bool compress_warp(const __half *__restrict__ x, int6
     }
     __syncwarp();
     if (valid) {
-        uint8_t *dst = blocks + (b * bs_b + h * bs_h + l) * rec;
+        uint8_t *dst = kGiven ? given_dst : blocks + (b * bs_b + h * bs_h + l) * rec;
         const uint4 w0 = *reinterpret_cast<const uint4 *>(st + 4 * g);
         uint4 w1;
         if (g == 0) {
@@ -412,6 +427,12 @@ __device__ __noinline__ void compress_warp_exact(const __half *__restrict__ x, i
                                                  int64_t bs_h, FastDiv div_h, FastDiv div_l, uint32_t n_vec,
                                                  uint32_t tile, const QEntry *tab, uint32_t *st, uint32_t rec) {
     compress_warp<kRotate, true>(x, xs_b, xs_h, xs_l, blocks, bs_b, bs_h, div_h, div_l, n_vec, tile, tab, st, rec);
+}
+template <bool kRotate>
+__device__ __noinline__ void compress_warp_exact_paged(const CompressJob &jb, uint32_t tile, const QEntry *tab,
+                                                       uint32_t *st, uint8_t *dst, bool valid) {
+    compress_warp<kRotate, true, true>(jb.x, jb.xs_b, jb.xs_h, jb.xs_l, nullptr, 0, 0, jb.div_h, jb.div_l, jb.n_vec,
+                                       tile, tab, st, jb.rec, dst, valid);
 }
 
 // ---- packed fast pass -------------------------------------------------------
@@ -482,8 +503,9 @@ struct VecRef {
     bool tail;     // this lane also writes bytes 64 + 16g.. of the block (false for the pad sector of a 96-byte record)
 };
 
+// `pages`: the destination is looked up in a page table.
 __device__ __forceinline__ void load_vec(const CompressJob &jb, uint32_t tile, uint4 (&raw)[4], VecRef &ref,
-                                         int64_t off = 0, bool enabled = true) {
+                                         int64_t off = 0, bool enabled = true, const PagedJobs *pages = nullptr) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane & 3, vsub = lane >> 2;
     const uint32_t vi = tile * kVecPerTile + warp * kVecPerWarp + vsub;
@@ -494,7 +516,10 @@ __device__ __forceinline__ void load_vec(const CompressJob &jb, uint32_t tile, u
     const uint32_t bq = fdiv(row, jb.div_h);
     const int64_t b = bq, h = row - bq * jb.div_h.d;
     const __half *src = jb.x + b * jb.xs_b + h * jb.xs_h + l * jb.xs_l + 8 * g;
-    ref.dst = jb.blocks + off + (b * jb.bs_b + h * jb.bs_h + l) * jb.rec;
+    if (pages)
+        ref.valid = ref.valid && paged_dst(*pages, jb, (int)b, h, l, ref.dst);
+    else
+        ref.dst = jb.blocks + off + (b * jb.bs_b + h * jb.bs_h + l) * jb.rec;
     ref.tail = 64 + 16 * g < (int)jb.rec;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -710,8 +735,9 @@ __device__ __forceinline__ bool compress_fast(const uint4 (&raw)[4], const VecRe
     return true;
 }
 
-template <bool kRotate>
-__global__ void __launch_bounds__(kCompressWarps * 32, 3) compress_kernel(const __grid_constant__ CompressJobs jobs) {
+template <bool kRotate, class Jobs>
+__global__ void __launch_bounds__(kCompressWarps * 32, 3) compress_kernel(const __grid_constant__ Jobs jobs) {
+    constexpr bool kPaged = std::is_same<Jobs, PagedJobs>::value;
     __shared__ QEntry tab[kCells * kReplicas];
     __shared__ __align__(16) uint32_t stage[kCompressWarps][kVecPerWarp][20];
     __shared__ __align__(16) float reduce[kCompressWarps][kVecPerWarp][40];
@@ -729,29 +755,34 @@ __global__ void __launch_bounds__(kCompressWarps * 32, 3) compress_kernel(const 
     int64_t off0, off1 = 0;
     const bool en0 = job_offset(jobs.j[0], off0);
     const bool en1 = jobs.njobs > 1 ? job_offset(jobs.j[1], off1) : true;
+    const PagedJobs *pages = nullptr;
+    if constexpr (kPaged) pages = &jobs;
     // the next tile's inputs are loaded before the current tile is processed
     uint32_t tile = blockIdx.x;
     uint4 raw[4];
     VecRef ref;
     if (tile < n_tiles) {
-        if (tile >= t0) load_vec(jobs.j[1], tile - t0, raw, ref, off1, en1);
-        else load_vec(jobs.j[0], tile, raw, ref, off0, en0);
+        if (tile >= t0) load_vec(jobs.j[1], tile - t0, raw, ref, off1, en1, pages);
+        else load_vec(jobs.j[0], tile, raw, ref, off0, en0, pages);
     }
     while (tile < n_tiles) {
         const uint32_t next = tile + gridDim.x;
         uint4 nraw[4];
         VecRef nref;
         if (next < n_tiles) {
-            if (next >= t0) load_vec(jobs.j[1], next - t0, nraw, nref, off1, en1);
-            else load_vec(jobs.j[0], next, nraw, nref, off0, en0);
+            if (next >= t0) load_vec(jobs.j[1], next - t0, nraw, nref, off1, en1, pages);
+            else load_vec(jobs.j[0], next, nraw, nref, off0, en0, pages);
         }
         if (!compress_fast<kRotate>(raw, ref, tabq, red, st)) {
             const bool second = tile >= t0;  // block-uniform
             const CompressJob &jb = second ? jobs.j[1] : jobs.j[0];
             const uint32_t t = second ? tile - t0 : tile;
-            compress_warp_exact<kRotate>(jb.x, jb.xs_b, jb.xs_h, jb.xs_l, jb.blocks + (second ? off1 : off0), jb.bs_b,
-                                         jb.bs_h, jb.div_h, jb.div_l, (second ? en1 : en0) ? jb.n_vec : 0u, t, tab,
-                                         st, jb.rec);
+            if constexpr (kPaged)
+                compress_warp_exact_paged<kRotate>(jb, t, tab, st, ref.dst, ref.valid);
+            else
+                compress_warp_exact<kRotate>(jb.x, jb.xs_b, jb.xs_h, jb.xs_l, jb.blocks + (second ? off1 : off0),
+                                             jb.bs_b, jb.bs_h, jb.div_h, jb.div_l,
+                                             (second ? en1 : en0) ? jb.n_vec : 0u, t, tab, st, jb.rec);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) raw[c] = nraw[c];
@@ -795,8 +826,9 @@ __device__ __forceinline__ float tsum_warp(const float (&v)[4], int lane) {
     return s;
 }
 
-template <bool kRotate>
-__global__ void __launch_bounds__(kLatWarps * 32) compress_lat_kernel(const __grid_constant__ CompressJobs jobs) {
+template <bool kRotate, class Jobs>
+__global__ void __launch_bounds__(kLatWarps * 32) compress_lat_kernel(const __grid_constant__ Jobs jobs) {
+    constexpr bool kPaged = std::is_same<Jobs, PagedJobs>::value;
     __shared__ QEntry tab[kCells * kReplicas];
     build_qtable(tab);
     __syncthreads();
@@ -819,6 +851,12 @@ __global__ void __launch_bounds__(kLatWarps * 32) compress_lat_kernel(const __gr
     const int64_t l = vi - row * jb.div_l.d;
     const uint32_t bq = fdiv(row, jb.div_h);
     const int64_t b = bq, h = row - bq * jb.div_h.d;
+    uint8_t *dst = nullptr;
+    if constexpr (kPaged) {
+        if (!paged_dst(jobs, jb, (int)b, h, l, dst)) return;  // warp-uniform
+    } else {
+        dst = jb.blocks + (second ? off1 : off0) + (b * jb.bs_b + h * jb.bs_h + l) * jb.rec;
+    }
 
     float v[4];
     {
@@ -949,7 +987,6 @@ __global__ void __launch_bounds__(kLatWarps * 32) compress_lat_kernel(const __gr
     } else if (lane == 21) {
         word = (uint32_t)__half_as_ushort(__float2half_rn(alpha));
     }
-    uint8_t *dst = jb.blocks + (second ? off1 : off0) + (b * jb.bs_b + h * jb.bs_h + l) * jb.rec;
     if (4 * lane < (int)jb.rec) reinterpret_cast<uint32_t *>(dst)[lane] = word;
 }
 
@@ -1175,8 +1212,8 @@ static int dev_info(DevInfo **out) {
         int sms = 0;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return ECC_ERR_DEVICE;
         int a = 0, b = 0;
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&a, compress_kernel<false>, kCompressWarps * 32, 0);
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, compress_kernel<true>, kCompressWarps * 32, 0);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&a, compress_kernel<false, CompressJobs>, kCompressWarps * 32, 0);
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&b, compress_kernel<true, CompressJobs>, kCompressWarps * 32, 0);
         di.compress_ctas_per_sm[0] = std::max(a, 1);
         di.compress_ctas_per_sm[1] = std::max(b, 1);
         di.sms = sms;
@@ -1232,7 +1269,8 @@ static int make_job(const void *x_f16, int64_t xs_b, int64_t xs_h, int64_t xs_l,
     return ECC_OK;
 }
 
-static int launch_jobs(CompressJobs &jobs, int mode, ecc_stream_t stream) {
+template <class Jobs>
+static int launch_jobs(Jobs &jobs, int mode, ecc_stream_t stream) {
     const bool rotate = (mode & ECC_COMPRESS_ROTATE) != 0;
     // drop empty jobs
     if (jobs.njobs > 1 && jobs.j[1].n_vec == 0) jobs.njobs = 1;
@@ -1248,17 +1286,17 @@ static int launch_jobs(CompressJobs &jobs, int mode, ecc_stream_t stream) {
     const int64_t nvec = (int64_t)jobs.j[0].n_vec + (jobs.njobs > 1 ? jobs.j[1].n_vec : 0);
     if (nvec <= kLatencyMaxVectors) {  // appends: one warp per vector
         const dim3 grid((unsigned)((nvec + kLatWarps - 1) / kLatWarps)), block(kLatWarps * 32);
-        const cudaError_t e = rotate ? launch_pdl(compress_lat_kernel<true>, grid, block, 0, s, jobs)
-                                     : launch_pdl(compress_lat_kernel<false>, grid, block, 0, s, jobs);
+        const cudaError_t e = rotate ? launch_pdl(compress_lat_kernel<true, Jobs>, grid, block, 0, s, jobs)
+                                     : launch_pdl(compress_lat_kernel<false, Jobs>, grid, block, 0, s, jobs);
         if (e != cudaSuccess) return ECC_ERR_LAUNCH;
         return launch_status();
     }
     const int64_t tiles = (int64_t)jobs.j[0].n_tiles + (jobs.njobs > 1 ? jobs.j[1].n_tiles : 0);
     if (tiles >= (int64_t)0xffffff00ll) return ECC_ERR_SHAPE;
     const int64_t grid = std::min<int64_t>(tiles, (int64_t)di->sms * di->compress_ctas_per_sm[rotate ? 1 : 0]);
-    const cudaError_t e = rotate ? launch_pdl(compress_kernel<true>, dim3((unsigned)grid), dim3(kCompressWarps * 32),
+    const cudaError_t e = rotate ? launch_pdl(compress_kernel<true, Jobs>, dim3((unsigned)grid), dim3(kCompressWarps * 32),
                                               0, s, jobs)
-                                 : launch_pdl(compress_kernel<false>, dim3((unsigned)grid),
+                                 : launch_pdl(compress_kernel<false, Jobs>, dim3((unsigned)grid),
                                               dim3(kCompressWarps * 32), 0, s, jobs);
     if (e != cudaSuccess) return ECC_ERR_LAUNCH;
     return launch_status();
@@ -1370,7 +1408,42 @@ extern "C" int ecc_compress_strided_calibrated_at(const void *x_f16, int64_t xs_
                                     pos_dev, capacity, stream);
 }
 
+extern "C" int ecc_compress_paged(const void *x0_f16, int64_t x0s_b, int64_t x0s_h, int64_t x0s_l, void *blocks0,
+                                  int64_t b0s_p, int64_t b0s_h, const void *x1_f16, int64_t x1s_b, int64_t x1s_h,
+                                  int64_t x1s_l, void *blocks1, int64_t b1s_p, int64_t b1s_h, int B, int H, int64_t L,
+                                  const ecc_pages_t *pages, const int *pos, const int *new_lens, int rotate,
+                                  ecc_stream_t stream) {
+    if (!pages || !pos) return ECC_ERR_NULL;
+    if (!aligned(pos, 4) || !aligned(new_lens, 4)) return ECC_ERR_ALIGN;
+    if (L > (1ll << 30)) return ECC_ERR_SHAPE;
+    PagedJobs jobs{};
+    int rc = paged::make_table(*pages, &jobs.t);
+    if (rc != ECC_OK) return rc;
+    jobs.pos = pos;
+    jobs.new_lens = new_lens;
+    int64_t n0 = 0, n1 = 0;
+    rc = make_job(x0_f16, x0s_b, x0s_h, x0s_l, blocks0, b0s_p, b0s_h, B, H, L, rotate, &jobs.j[0], &n0);
+    if (rc != ECC_OK) return rc;
+    jobs.njobs = 1;
+    if (x1_f16 || blocks1) {
+        rc = make_job(x1_f16, x1s_b, x1s_h, x1s_l, blocks1, b1s_p, b1s_h, B, H, L, rotate, &jobs.j[1], &n1);
+        if (rc != ECC_OK) return rc;
+        jobs.njobs = 2;
+    }
+    if (n0 == 0) return ECC_OK;
+    return launch_jobs(jobs, rotate, stream);
+}
+
 namespace ecc {
+int compress_paged_error(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, paged::g_paged_error, sizeof(int)) != cudaSuccess) return ECC_ERR_CUDA;
+    if (reset) {
+        const int z = 0;
+        if (cudaMemcpyToSymbol(paged::g_paged_error, &z, sizeof(int)) != cudaSuccess) return ECC_ERR_CUDA;
+    }
+    return v;
+}
 int compress_device_error(int reset) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_compress_error, sizeof(int)) != cudaSuccess) return ECC_ERR_CUDA;

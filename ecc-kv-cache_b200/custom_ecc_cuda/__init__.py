@@ -30,7 +30,8 @@ __all__ = [
     "compress_pair_at", "compress_calibrated_at", "decode_attention_dev", "decode_dev_workspace_size",
     "decode_partials_dev", "decode_dev_splits", "exchange_buffer_bytes", "lse_exchange_merge",
     "exchange_alloc", "exchange_open", "exchange_close", "exchange_free", "lse_gather_merge",
-    "decode_attention_masked",
+    "decode_attention_masked", "compress_pair_paged", "dequantize_paged", "decode_attention_paged",
+    "decode_paged_workspace_size",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -51,6 +52,12 @@ RECORD96 = 96          # the block without its zero pad sector (bytes 96..127)
 
 class EccError(RuntimeError):
     """A negative status from libeccb200.so."""
+
+
+class _Pages(ctypes.Structure):
+    """ecc_pages_t"""
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("width", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("n_pages", ctypes.c_int64)]
 
 
 def _load():
@@ -102,6 +109,12 @@ def _load():
         "ecc_lse_gather_merge": ([p, p, p, i64, i32, i32, p, i32, i32, ctypes.c_uint32, ctypes.c_longlong, p, i32,
                                   p], i32),
         "ecc_lse_exchange_merge_dev": ([p, p, p, i64, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
+        "ecc_compress_paged": ([p, i64, i64, i64, p, i64, i64, p, i64, i64, i64, p, i64, i64, i32, i32, i64, p, p, p,
+                                i32, p], i32),
+        "ecc_dequantize_paged": ([p, i64, i64, p, p, i64, i64, p, i32, i32, i64, p, p, i32, p], i32),
+        "ecc_decode_paged_workspace_size": ([i32, i32, i32, i64, i32], sz),
+        "ecc_decode_paged": ([p, p, p, i64, i64, p, p, p, p, p, i64, i64, p, sz, i32, i32, i32, f32, i32, i32, i32, p],
+                             i32),
         "ecc_lse_gather_merge_dev": ([p, p, p, i64, i32, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
     }
     for name, (args, res) in sig.items():
@@ -721,7 +734,8 @@ def device_status(reset: bool = False) -> int:
     hanging), 2 if the decode kernel found its shared memory at an unexpected
     address (it computed nothing), 3 if an append at a device-side position
     was out of range (it wrote nothing), 4 if lse_exchange_merge gave up
-    waiting for another rank's records (those rows were not written), else 0."""
+    waiting for another rank's records (those rows were not written), 5 if a
+    call on a paged cache met a length, position or page out of range, else 0."""
     rc = int(_lib.ecc_device_status(1 if reset else 0))
     if rc < 0:
         _check(rc, "device_status")
@@ -856,3 +870,164 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                                           _stream(q3))
     _check(rc, "decode_partials_dev")
     return pm, pl, po
+
+
+# ---------------------------------------------------------------------------
+# Paged cache: sequences of any lengths in pages of a shared pool
+# ---------------------------------------------------------------------------
+def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_table: torch.Tensor, B: int):
+    """Checks pools [pages, Hkv, page_size, R] and their page table [B, width]
+    int32; returns ((k strides), (v strides), ecc_pages_t)."""
+    ks = _pool_strides(k_pool, "k_pool")
+    if k_pool.dim() != 4:
+        raise RuntimeError("a paged pool must be [pages, Hkv, page_size, 128] (or [.., 96])")
+    vs = ks
+    if v_pool is not None:
+        vs = _pool_strides(v_pool, "v_pool")
+        if v_pool.shape != k_pool.shape or v_pool.device != k_pool.device:
+            raise RuntimeError("k_pool and v_pool must have the same shape and device")
+    _dev_int(block_table, "block_table", k_pool.device)
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1:
+        raise RuntimeError("block_table must be int32 [B, width] with contiguous rows, one row per sequence")
+    P, ps, width = k_pool.shape[0], k_pool.shape[2], block_table.shape[1]
+    if ps % 16 and width > 1:
+        raise RuntimeError(f"page_size must be a multiple of 16 (or one page per sequence), got {ps}")
+    return ks, vs, _Pages(block_table.data_ptr(), block_table.stride(0), width, ps, P)
+
+
+def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> None:
+    _dev_int(t, name, device)
+    if t.dim() != 1 or t.numel() != B or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of B elements")
+
+
+def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
+                        block_table: torch.Tensor, pos: torch.Tensor, new_lens: torch.Tensor | None = None,
+                        rotate: bool = True) -> None:
+    """compress_pair_into for a paged cache: token i of sequence b of ``k``,
+    ``v`` [B, Hkv, L, 128] fp16 goes to position ``pos[b] + i`` (int32 [B] on
+    the GPU), that is to page ``block_table[b, p // page_size]``, slot ``p %
+    page_size`` of the pools [pages, Hkv, page_size, 128 or 96].  With
+    ``new_lens`` (int32 [B] on the GPU) only the first new_lens[b] tokens of a
+    sequence are written, the rest of the row is padding.  ``v``/``v_pool``
+    None: ``k`` alone.  A position or page out of range writes nothing and
+    raises the flag device_status() reports; two tokens of one call must not
+    name the same slot."""
+    if k.dim() != 4:
+        raise RuntimeError("k must be float16 [B, Hkv, L, 128]")
+    if (v is None) != (v_pool is None):
+        raise RuntimeError("v and v_pool go together")
+    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, k.shape[0])
+    for t, name in ((k, "k"), (v, "v")):
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dtype != torch.float16 or t.shape[-1] != D or t.stride(-1) != 1 or t.shape != k.shape:
+            raise RuntimeError(f"{name} must be float16 [B, Hkv, L, 128] with a contiguous last dimension, k and v alike")
+        if t.shape[1] != k_pool.shape[1] or t.device != k_pool.device:
+            raise RuntimeError(f"{name} must have the pools' kv heads and device")
+    B, H, L, _ = k.shape
+    _per_sequence(pos, "pos", k.device, B)
+    if new_lens is not None:
+        _per_sequence(new_lens, "new_lens", k.device, B)
+    vargs = (None, 0, 0, 0, None, 0, 0) if v is None else (_ptr(v), v.stride(0), v.stride(1), v.stride(2),
+                                                           _ptr(v_pool), vs[0], vs[1])
+    with torch.cuda.device(k.device):
+        rc = _lib.ecc_compress_paged(_ptr(k), k.stride(0), k.stride(1), k.stride(2), _ptr(k_pool), ks[0], ks[1], *vargs,
+                                     B, H, L, ctypes.byref(pages), _ptr(pos),
+                                     None if new_lens is None else _ptr(new_lens), _cmode(rotate, k_pool, v_pool),
+                                     _stream(k))
+    _check(rc, "compress_pair_paged")
+
+
+def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_table: torch.Tensor,
+                     seq_lens: torch.Tensor, max_len: int, unrotate: bool = True, out: tuple | None = None):
+    """Reads a paged context back: (k, v), each [B, Hkv, max_len, 128] fp16,
+    the first min(seq_lens[b], max_len) tokens of every sequence and zeros
+    behind them, with the inverse rotation applied (``unrotate``; one rounding
+    at the end).  ``v_pool`` None gives k alone.  ``out``: tensors to write to,
+    contiguous and of that shape."""
+    B = block_table.shape[0]
+    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
+    _per_sequence(seq_lens, "seq_lens", k_pool.device, B)
+    H, dev, n = k_pool.shape[1], k_pool.device, 1 if v_pool is None else 2
+    shape = (B, H, int(max_len), D)
+    if max_len < 0:
+        raise RuntimeError("max_len must not be negative")
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=torch.float16, device=dev) for _ in range(n))
+    elif len(out) != n or any(tuple(t.shape) != shape or t.dtype != torch.float16 or not t.is_contiguous()
+                              or t.device != dev for t in out):
+        raise RuntimeError("out must hold contiguous float16 tensors [B, Hkv, max_len, 128] on the pools' device")
+    mode = (1 if unrotate else 0) | (2 if k_pool.shape[-1] == RECORD96 else 0)
+    with torch.cuda.device(dev):
+        rc = _lib.ecc_dequantize_paged(_ptr(k_pool), ks[0], ks[1], _ptr(out[0]),
+                                       None if v_pool is None else _ptr(v_pool), vs[0], vs[1],
+                                       None if v_pool is None else _ptr(out[1]), B, H, int(max_len),
+                                       ctypes.byref(pages), _ptr(seq_lens), mode, _stream(k_pool))
+    _check(rc, "dequantize_paged")
+    return out if v_pool is not None else out[0]
+
+
+def decode_paged_workspace_size(B: int, hq: int, hkv: int, capacity: int, with_weights: bool = False) -> int:
+    """Workspace bytes of decode_attention_paged for tables that can name
+    ``capacity`` = width * page_size tokens."""
+    return int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(bool(with_weights))))
+
+
+def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                           seq_lens: torch.Tensor, sm_scale: float | None = None, window: int = 0, sinks: int = 0,
+                           rotate_q: bool = False, unrotate_out: bool = False, weights: torch.Tensor | None = None,
+                           return_lse: bool = False, out: torch.Tensor | None = None,
+                           workspace: torch.Tensor | None = None):
+    """decode_attention over a paged cache: sequence b of ``query`` [B, Hq, 1,
+    128] attends to its first ``seq_lens[b]`` tokens (int32 [B] on the GPU,
+    read when the kernel runs) in the pages ``block_table[b]`` (int32 [B,
+    width]) of the pools [pages, Hkv, page_size, 128 or 96].
+
+    ``window`` > 0: only the last ``window`` tokens and the first ``sinks`` are
+    visible.  ``weights`` (fp32 [B, Hkv, >= width * page_size], contiguous last
+    dim): every visible token's softmax weight, summed over the group's query
+    heads, is added to it in place.  ``return_lse``: also the natural log of
+    each row's sum of e^score, [B, Hq] fp32.  A sequence of length 0 gives a
+    zero row (lse -inf) and adds no weight.  GQA groups of up to 8."""
+    q3 = _query(query)
+    B, hq, _ = q3.shape
+    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
+    if ks != vs:
+        raise RuntimeError("k_pool and v_pool must have the same strides")
+    dev, hkv = k_pool.device, k_pool.shape[1]
+    if q3.device != dev:
+        raise RuntimeError("query and pools must be on the same device")
+    if hq % hkv or hq // hkv > 8:
+        raise RuntimeError(f"query heads ({hq}) must be 1 to 8 times the kv heads ({hkv})")
+    _per_sequence(seq_lens, "seq_lens", dev, B)
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise RuntimeError("window and sinks must not be negative, and sinks need a window")
+    capacity = pages.width * pages.page_size
+    wargs = (None, 0, 0)
+    if weights is not None:
+        _require_cuda(weights, "weights")
+        if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, hkv) \
+                or weights.shape[2] < capacity or weights.stride(2) != 1 or weights.device != dev:
+            raise RuntimeError(f"weights must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on "
+                               f"the pools' device")
+        wargs = (_ptr(weights), weights.stride(0), weights.stride(1))
+    if out is None:
+        out = torch.empty((B, hq, 1, D), dtype=torch.float16, device=dev)
+    elif not out.is_contiguous() or out.dtype != torch.float16 or out.numel() != B * hq * D or out.device != dev:
+        raise RuntimeError("out must be a contiguous float16 tensor of B*Hq*128 elements on the pools' device")
+    lse = torch.empty((B, hq), dtype=torch.float32, device=dev) if return_lse else None
+    flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | _rec_flag(k_pool)
+    need = int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(weights is not None)))
+    with torch.cuda.device(dev):
+        ws = workspace if workspace is not None else _workspace(dev, need)
+        if ws.numel() * ws.element_size() < need or ws.device != dev:
+            raise RuntimeError(f"workspace too small or on another device: {need} bytes needed")
+        rc = _lib.ecc_decode_paged(_ptr(q3), _ptr(k_pool), _ptr(v_pool), ks[0], ks[1], ctypes.byref(pages),
+                                   _ptr(seq_lens), _ptr(out), None if lse is None else _ptr(lse), *wargs, _ptr(ws),
+                                   ws.numel() * ws.element_size(), B, hq, hkv,
+                                   float(sm_scale) if sm_scale is not None else 0.0, int(window), int(sinks), flags,
+                                   _stream(q3))
+    _check(rc, "decode_attention_paged")
+    return (out, lse) if return_lse else out

@@ -79,8 +79,9 @@ int ecc_version(void);
  *   3  an append at a device-side position (ecc_compress_strided_pair_at,
  *      ..._calibrated_at) was out of range and wrote nothing;
  *   4  ecc_lse_exchange_merge ran out of its wait for another rank's records
- *      (the rows it waited for were not written).
- * When several were raised, the lowest of 1/2 (decode), 3, 4 is returned. */
+ *      (the rows it waited for were not written);
+ *   5  a call on a paged cache met a length, position or page out of range.
+ * When several were raised, the lowest of 1/2 (decode), 3, 4, 5 is returned. */
 int ecc_device_status(int reset);
 
 /* Self-test of the bounded device waits (no counterpart in the reference):
@@ -378,6 +379,68 @@ int ecc_lse_gather_merge_dev(const float *part_m, const float *part_l, const flo
 int ecc_decode_static(const void *q_f16, const void *k_blocks, const void *v_blocks, int64_t bs_b,
                       int64_t bs_h, void *out_f16, int B, int Hq, int Hkv, int64_t seq_len,
                       float sm_scale, int flags, int num_splits, ecc_stream_t stream);
+
+/* ---- paged cache ----------------------------------------------------------
+ * Pools in pages: block (page, kv head, slot) at block index page*bs_p +
+ * kv_head*bs_h + slot (blocks or 96-byte records).  Token t of sequence b lies
+ * in page table[b*table_stride + t / page_size] at slot t % page_size; pages
+ * may be shared between sequences that only read them.  Lengths and positions
+ * are DEVICE int32 arrays, read when the kernel runs, so one recorded launch
+ * serves a growing cache.  No counterpart in the reference, whose cache holds
+ * one contiguous row per sequence and one length for all of them.
+ *   table: DEVICE int32; entries behind a sequence's last page are not read.
+ *   width: columns of the table; page_size: a multiple of 16, or any size when
+ *   width is 1; n_pages: pages of the pools; width * page_size <= 2^30.
+ * A length, position or page out of range raises ecc_device_status 5: nothing
+ * is read or written out of bounds, the tokens concerned are not written, and
+ * the output of the sequence concerned is not valid. */
+typedef struct {
+    const int *table;
+    int64_t table_stride;
+    int width;
+    int page_size;
+    int64_t n_pages;
+} ecc_pages_t;
+
+/* ecc_compress_strided_pair into pages: token l of sequence b goes to position
+ * pos[b] + l, for l < new_lens[b] (every l < L when new_lens is NULL).  x1_f16
+ * = blocks1 = NULL: one tensor.  Two tokens of one call must not name the same
+ * slot (the block written would be one of the two, or a mixture). */
+int ecc_compress_paged(const void *x0_f16, int64_t x0s_b, int64_t x0s_h, int64_t x0s_l, void *blocks0, int64_t b0s_p,
+                       int64_t b0s_h, const void *x1_f16, int64_t x1s_b, int64_t x1s_h, int64_t x1s_l, void *blocks1,
+                       int64_t b1s_p, int64_t b1s_h, int B, int H, int64_t L, const ecc_pages_t *pages, const int *pos,
+                       const int *new_lens, int rotate, ecc_stream_t stream);
+
+/* Reads a paged context back: out[b][h][t] (contiguous [B, H, max_len, 128]
+ * fp16) = the reconstruction (C[q]*scale + zero) + alpha*s of token t, with
+ * the inverse rotation applied in fp32 when ECC_DEQUANT_UNROTATE is set and
+ * one rounding at the end; zero for t >= seq_lens[b].  blocks1 = out1 = NULL:
+ * one pool.  ECC_DEQUANT_BLOCK96: 96-byte records. */
+#define ECC_DEQUANT_UNROTATE 1
+#define ECC_DEQUANT_BLOCK96 2
+int ecc_dequantize_paged(const void *blocks0, int64_t b0s_p, int64_t b0s_h, void *out0_f16, const void *blocks1,
+                         int64_t b1s_p, int64_t b1s_h, void *out1_f16, int B, int H, int64_t max_len,
+                         const ecc_pages_t *pages, const int *seq_lens, int mode, ecc_stream_t stream);
+
+/* ecc_decode over pages: sequence b attends to its first seq_lens[b] tokens;
+ * with window > 0 only to the last `window` of them and the first `sinks`.
+ * An empty sequence gives a zero row.
+ *   lse: [B, Hq] fp32, natural log of the row's sum of e^score (-inf for an
+ *     empty row), or NULL.
+ *   weights: fp32 accumulators, element (b, kv head, t) at b*ws_b + h*ws_h + t,
+ *     for every t below the table's width * page_size: each visible token's
+ *     softmax weight, summed over the group's query heads, is added to it; or
+ *     NULL.
+ *   workspace: ecc_decode_paged_workspace_size() bytes (which 0 says that the
+ *     sizes are out of range); capacity = width * page_size.
+ * GQA groups up to 8, B up to ECC_PAGED_MAX_BATCH; flags: ECC_DECODE_ROTATE_Q,
+ * ECC_DECODE_UNROTATE_OUT, ECC_DECODE_BLOCK96. */
+#define ECC_PAGED_MAX_BATCH 4096
+size_t ecc_decode_paged_workspace_size(int B, int Hq, int Hkv, int64_t capacity, int with_weights);
+int ecc_decode_paged(const void *q_f16, const void *k_blocks, const void *v_blocks, int64_t bs_p, int64_t bs_h,
+                     const ecc_pages_t *pages, const int *seq_lens, void *out_f16, float *lse, float *weights,
+                     int64_t ws_b, int64_t ws_h, void *workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
+                     float sm_scale, int window, int sinks, int flags, ecc_stream_t stream);
 
 #ifdef __cplusplus
 }
