@@ -1,0 +1,224 @@
+// cluster_select.cuh -- selection over one long row by a cluster of CTAs
+// (sm_100a): each CTA holds a contiguous slice of the row, the counts of the
+// slices are joined through distributed shared memory and the hardware
+// cluster barrier.  Used by the cache eviction and by sampling.
+//
+// The k largest 32-bit keys of a row are found by a radix descent: per pass
+// the keys that match the prefix so far are counted by their next digit (up
+// to 11 bits), the cluster's counts are summed, and the digit in which the
+// k-th key falls extends the prefix.  Shared-memory atomics of one warp on
+// one address are serialised, so each bin has four copies, picked by lane.
+#pragma once
+#include <cooperative_groups.h>
+
+#include "ecc_common.cuh"
+
+namespace ecc {
+namespace sel {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kCopies = 4;
+constexpr int kPerThread = kBins / kThreads;
+constexpr int kMaxCluster = 16;
+
+struct alignas(16) Shared {
+    uint32_t hist[kBins * kCopies];
+    uint32_t sum[kBins];  // this CTA's counts of a pass, read by the cluster
+    uint32_t warp_a[kWarps], warp_b[kWarps];
+    uint64_t warp64[kWarps];
+    uint32_t cta_a, cta_b;  // totals of this CTA, read by the cluster
+    uint64_t cta64;
+    uint32_t found[3];
+    uint64_t found64[2];
+    uint32_t cut;  // written by the CTA that finds it
+};
+
+// Ascending order of floats as ascending unsigned order; -0 equals +0.
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <class T>
+__device__ __forceinline__ T *of_rank(cg::cluster_group &cl, T *p, unsigned rank) {
+    return cl.map_shared_rank(p, rank);
+}
+
+// Exclusive prefix of v over the block's threads; *total = the sum.
+template <class T>
+__device__ __forceinline__ T block_exclusive(T v, T *warp_sums, T *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    __syncthreads();  // earlier readers of warp_sums are done
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    T before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const T x = warp_sums[w];
+        before += w < warp ? x : 0;
+        all += x;
+    }
+    *total = all;
+    return before + inc - v;
+}
+
+// The k-th largest key of the cluster's row, 1 <= k <= keys of the row.
+// keys(i), i < n, are this CTA's; passes of `bits` bits from bit 31 down to
+// bit `low` (the bits below are zero in every key).  *ties: how many of the
+// keys equal to it belong to the k largest; *equal: how many there are.
+template <class Keys>
+__device__ __forceinline__ uint32_t kth_largest(Shared &sh, cg::cluster_group &cl, const Keys &keys, int n, uint32_t k,
+                                                int low, uint32_t *ties, uint32_t *equal) {
+    const int tid = threadIdx.x;
+    const unsigned ranks = cl.num_blocks();
+    uint32_t prefix = 0, mask = 0;
+    int top = 32;
+    while (top > low) {
+        const int bits = min(11, top - low), shift = top - bits;
+        const uint32_t bins = 1u << bits;
+        for (int i = tid; i < kBins * kCopies; i += kThreads) sh.hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            const uint32_t x = keys(i);
+            if ((x & mask) == prefix) atomicAdd(&sh.hist[((x >> shift) & (bins - 1)) * kCopies + (tid & (kCopies - 1))], 1u);
+        }
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kThreads)
+            sh.sum[i] = (sh.hist[4 * i] + sh.hist[4 * i + 1]) + (sh.hist[4 * i + 2] + sh.hist[4 * i + 3]);
+        cl.sync();
+        // thread t takes bins from the top: kBins - 1 - 4t and the three below
+        uint32_t c[kPerThread], mine = 0;
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            const int bin = kBins - 1 - (tid * kPerThread + j);
+            c[j] = 0;
+            for (unsigned r = 0; r < ranks; ++r) c[j] += of_rank(cl, sh.sum, r)[bin];
+            mine += c[j];
+        }
+        uint32_t all;
+        uint32_t before = block_exclusive(mine, sh.warp_a, &all);
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            if (before < k && k <= before + c[j]) {
+                sh.found[0] = kBins - 1 - (tid * kPerThread + j);
+                sh.found[1] = before;
+                sh.found[2] = c[j];
+            }
+            before += c[j];
+        }
+        cl.sync();  // found is written; every CTA has read the sums
+        prefix |= sh.found[0] << shift;
+        mask |= (bins - 1) << shift;
+        k -= sh.found[1];
+        *equal = sh.found[2];
+        top = shift;
+        __syncthreads();
+    }
+    *ties = k;
+    return prefix;
+}
+
+// A warp's contiguous part of the CTA's n elements.
+__device__ __forceinline__ void warp_part(int n, int &lo, int &hi) {
+    const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
+    lo = min(n, (int)(threadIdx.x >> 5) * per);
+    hi = min(n, lo + per);
+}
+
+// Number of this warp's elements that satisfy p(i).
+template <class Pred>
+__device__ __forceinline__ uint32_t warp_count(int lo, int hi, const Pred &p) {
+    uint32_t c = 0;
+    for (int i = lo + (int)(threadIdx.x & 31); i < hi; i += 32) c += p(i) ? 1u : 0u;
+    return __reduce_add_sync(0xffffffffu, c);
+}
+
+// Cluster-wide exclusive prefix of one count per warp, in row order.
+__device__ __forceinline__ uint32_t cluster_exclusive(Shared &sh, cg::cluster_group &cl, uint32_t warp_value) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = warp_value;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const uint32_t x = sh.warp_a[w];
+        before += w < warp ? x : 0;
+        all += x;
+    }
+    if (threadIdx.x == 0) sh.cta_a = all;
+    cl.sync();
+    for (unsigned r = 0; r < cl.block_rank(); ++r) before += *of_rank(cl, &sh.cta_a, r);
+    cl.sync();  // cta_a may be written again
+    return before;
+}
+
+// Row position behind the `ties`-th element (in row order) that satisfies
+// p(i): elements of equal key are kept below it.  base: row position of this
+// CTA's element 0.
+template <class Pred>
+__device__ __forceinline__ uint32_t tie_cut(Shared &sh, cg::cluster_group &cl, int n, int base, uint32_t ties,
+                                            const Pred &p) {
+    int lo, hi;
+    warp_part(n, lo, hi);
+    const uint32_t c = warp_count(lo, hi, p);
+    const uint32_t before = cluster_exclusive(sh, cl, c);
+    if (before < ties && ties <= before + c) {  // this warp holds it
+        const int lane = threadIdx.x & 31;
+        uint32_t seen = before;
+        for (int i0 = lo; i0 < hi; i0 += 32) {
+            const bool hit = i0 + lane < hi && p(i0 + lane);
+            const uint32_t m = __ballot_sync(0xffffffffu, hit);
+            if (hit && seen + __popc(m & ((1u << lane) - 1u)) + 1 == ties)
+                for (unsigned r = 0; r < cl.num_blocks(); ++r) *of_rank(cl, &sh.cut, r) = (uint32_t)(base + i0 + lane + 1);
+            seen += __popc(m);
+        }
+    }
+    cl.sync();
+    const uint32_t cut = sh.cut;
+    __syncthreads();
+    return cut;
+}
+
+// Cluster size for `rows` rows: the largest power of two up to `most` with
+// which every CTA still has an SM of its own.
+static inline int cluster_size(int64_t rows, int sms, int most) {
+    int c = 1;
+    while (c < most && rows * (2 * c) <= sms) c *= 2;
+    return c;
+}
+
+// Launch with a cluster of `c` CTAs per row (y), as a dependent of the kernel
+// before it on the stream.
+template <typename... KArgs, typename... Args>
+static inline cudaError_t launch_cluster(void (*kernel)(KArgs...), int c, int64_t rows, size_t smem, cudaStream_t s,
+                                         Args &&...args) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && c > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(c * rows));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)c, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+}  // namespace sel
+}  // namespace ecc

@@ -443,6 +443,7 @@ int exchange_device_error(int reset);
 int compress_paged_error(int reset);
 int paged_decode_error(int reset, int *wait_error);
 int paged_cache_error(int reset);
+int evict_error(int reset);
 }
 
 extern "C" int ecc_device_status(int reset) {
@@ -457,10 +458,12 @@ extern "C" int ecc_device_status(int reset) {
     const int x = ecc::exchange_device_error(reset);
     if (x < 0) return x;
     int w = 0;
-    const int p[3] = {ecc::paged_decode_error(reset, &w), ecc::compress_paged_error(reset),
-                      ecc::paged_cache_error(reset)};
-    for (int e : p)
+    int p = 0;
+    for (int e : {ecc::paged_decode_error(reset, &w), ecc::compress_paged_error(reset), ecc::paged_cache_error(reset),
+                  ecc::evict_error(reset)}) {
         if (e < 0) return e;
+        p = p ? p : e;
+    }
     if (!v) v = w;
-    return v ? v : c ? c : x ? x : p[0] ? p[0] : p[1] ? p[1] : p[2];
+    return v ? v : c ? c : x ? x : p;
 }

@@ -31,7 +31,7 @@ __all__ = [
     "decode_partials_dev", "decode_dev_splits", "exchange_buffer_bytes", "lse_exchange_merge",
     "exchange_alloc", "exchange_open", "exchange_close", "exchange_free", "lse_gather_merge",
     "decode_attention_masked", "compress_pair_paged", "dequantize_paged", "decode_attention_paged",
-    "decode_paged_workspace_size",
+    "decode_paged_workspace_size", "evict_paged", "sample_tokens",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -115,6 +115,10 @@ def _load():
         "ecc_decode_paged_workspace_size": ([i32, i32, i32, i64, i32], sz),
         "ecc_decode_paged": ([p, p, p, i64, i64, p, p, p, p, p, i64, i64, p, sz, i32, i32, i32, f32, i32, i32, i32, p],
                              i32),
+        "ecc_evict_paged_workspace_size": ([i64], sz),
+        "ecc_evict_paged": ([p, p, i64, i64, p, p, p, i64, i64, p, p, i64, i64, i64, p, i32, i32, i32, i32, i32, i32, p,
+                             sz, p], i32),
+        "ecc_sample": ([p, i64, i32, i32, i64, p, p, f32, p, i32, p, f32, p, f32, p, p, p], i32),
         "ecc_lse_gather_merge_dev": ([p, p, p, i64, i32, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
     }
     for name, (args, res) in sig.items():
@@ -1031,3 +1035,127 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
                                    _stream(q3))
     _check(rc, "decode_attention_paged")
     return (out, lse) if return_lse else out
+
+
+def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                weights: torch.Tensor, out_table: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
+                out_weights: torch.Tensor | None = None, kept: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None):
+    """Cuts the sequences of a paged cache down to ``budget`` tokens per kv
+    head by accumulated attention weight (``weights`` fp32 [B, Hkv, >=
+    capacity] of decode_attention_paged): a longer sequence keeps its first
+    ``sinks``, its last ``recent`` and the largest weights of the others (equal
+    ones: the earlier), in their order; a shorter one is kept whole.  The kept
+    blocks are copied to the pages ``out_table[b]`` (int32 [B, width], at least
+    ``budget`` tokens) of the same pools.  Those pages must be distinct and
+    hold no token of ``block_table``: otherwise device_status() reports 5 and
+    nothing is moved.
+
+    Returns (out_weights, kept): the kept tokens' weights with zeros behind
+    them, shaped as ``weights``, and int32 [B, Hkv, budget], the positions that
+    were kept (-1 behind them).  The new lengths are seq_lens.clamp(max=budget);
+    seq_lens itself is not changed, so that every layer can be cut by the same
+    lengths."""
+    B = block_table.shape[0]
+    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
+    ks2, _, outs = _paged_pools(k_pool, v_pool, out_table, B)
+    if ks != vs:
+        raise RuntimeError("k_pool and v_pool must have the same strides")
+    dev, hkv, capacity = k_pool.device, k_pool.shape[1], pages.width * pages.page_size
+    _per_sequence(seq_lens, "seq_lens", dev, B)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise RuntimeError("budget must be positive and hold the sinks and the recent tokens")
+    if outs.width * outs.page_size < budget:
+        raise RuntimeError(f"out_table names fewer than {budget} tokens per sequence")
+    if out_table.data_ptr() == block_table.data_ptr():
+        raise RuntimeError("out_table must name other pages than block_table")
+    if out_weights is None:
+        out_weights = torch.empty((B, hkv, weights.shape[-1]), dtype=torch.float32, device=dev)
+    for t, name in ((weights, "weights"), (out_weights, "out_weights")):
+        _require_cuda(t, name)
+        if t.dtype != torch.float32 or t.dim() != 3 or tuple(t.shape[:2]) != (B, hkv) or t.shape[2] < capacity \
+                or t.stride(2) != 1 or t.device != dev:
+            raise RuntimeError(f"{name} must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on the "
+                               f"pools' device")
+    if out_weights.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
+        raise RuntimeError("out_weights must not share memory with weights")
+    if kept is None:
+        kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
+    elif tuple(kept.shape) != (B, hkv, budget) or kept.dtype != torch.int32 or not kept.is_contiguous() \
+            or kept.device != dev:
+        raise RuntimeError("kept must be a contiguous int32 tensor [B, Hkv, budget] on the pools' device")
+    need = int(_lib.ecc_evict_paged_workspace_size(k_pool.shape[0]))
+    with torch.cuda.device(dev):
+        ws = workspace if workspace is not None else _workspace(dev, need)
+        if ws.numel() * ws.element_size() < need or ws.device != dev:
+            raise RuntimeError(f"workspace too small or on another device: {need} bytes needed")
+        rc = _lib.ecc_evict_paged(_ptr(k_pool), _ptr(v_pool), ks[0], ks[1], ctypes.byref(pages), _ptr(seq_lens),
+                                  _ptr(weights), weights.stride(0), weights.stride(1), ctypes.byref(outs),
+                                  _ptr(out_weights), out_weights.stride(0), out_weights.stride(1),
+                                  out_weights.shape[2], _ptr(kept), B, hkv, int(budget), int(sinks), int(recent),
+                                  k_pool.shape[-1], _ptr(ws), ws.numel() * ws.element_size(), _stream(k_pool))
+    _check(rc, "evict_paged")
+    return out_weights, kept
+
+
+# ---------------------------------------------------------------------------
+# Sampling
+# ---------------------------------------------------------------------------
+_SAMPLE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _setting(v, name: str, dtype, B: int, device, lo: float, hi: float):
+    """(device pointer or None, value) of a sampling setting: one value for
+    every row, or a [B] tensor on the GPU (whose values are not looked at)."""
+    if isinstance(v, torch.Tensor):
+        _require_cuda(v, name)
+        if v.dtype != dtype or tuple(v.shape) != (B,) or not v.is_contiguous() or v.device != device:
+            raise RuntimeError(f"{name} must be a number or a contiguous {dtype} tensor [B] on the logits' device")
+        return v.data_ptr(), 0
+    if not lo <= v <= hi:
+        raise RuntimeError(f"{name} must lie in [{lo}, {hi}], got {v}")
+    return None, v
+
+
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  return_logprobs: bool = False, out: torch.Tensor | None = None):
+    """The next token of every row of ``logits`` [B, V] (fp16, bf16 or fp32,
+    contiguous rows) from one given number in [0, 1) per row, ``uniform`` fp32
+    [B].  ``temperature`` divides the logits (0: the first maximum); ``top_k``
+    (0: off) keeps the k largest, ``top_p`` (1: off) the smallest set of the
+    largest that holds that share of the probability, ``min_p`` (0: off) those
+    with at least that share of the most likely one's; equal logits rank by
+    ascending index.  The token is the first, in ascending order, at which the
+    cumulative probability of the kept tokens exceeds the given number.  Each
+    setting is one number or a [B] tensor on the GPU (fp32; top_k int32).
+
+    Returns int64 [B]; with ``return_logprobs`` also fp32 [B], the log
+    probability of each token among the kept ones.  NaN logits count as -inf; a
+    row without a logit above -inf gives -1 (log probability -inf).  The draw is
+    computed to 2^-45 of the probabilities and does not depend on timing."""
+    _require_cuda(logits, "logits")
+    if logits.dim() != 2 or logits.dtype not in _SAMPLE_TYPES or logits.shape[1] < 1:
+        raise RuntimeError("logits must be float16, bfloat16 or float32 [B, V]")
+    B, V = logits.shape
+    dev = logits.device
+    if logits.stride(1) != 1 and V > 1:
+        raise RuntimeError("logits must have contiguous rows")
+    _require_cuda(uniform, "uniform")
+    if uniform.dtype != torch.float32 or tuple(uniform.shape) != (B,) or not uniform.is_contiguous() \
+            or uniform.device != dev:
+        raise RuntimeError("uniform must be a contiguous float32 tensor [B] on the logits' device")
+    t = _setting(temperature, "temperature", torch.float32, B, dev, 0.0, math.inf)
+    k = _setting(top_k, "top_k", torch.int32, B, dev, 0, 2 ** 31 - 1)
+    p = _setting(top_p, "top_p", torch.float32, B, dev, 2.0 ** -126, math.inf)
+    m = _setting(min_p, "min_p", torch.float32, B, dev, 0.0, 1.0)
+    if out is None:
+        out = torch.empty((B,), dtype=torch.int64, device=dev)
+    elif tuple(out.shape) != (B,) or out.dtype != torch.int64 or not out.is_contiguous() or out.device != dev:
+        raise RuntimeError("out must be a contiguous int64 tensor [B] on the logits' device")
+    logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprobs else None
+    with torch.cuda.device(dev):
+        rc = _lib.ecc_sample(_ptr(logits), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V, _ptr(uniform), t[0],
+                             float(t[1]), k[0], int(k[1]), p[0], float(p[1]), m[0], float(m[1]), _ptr(out),
+                             None if logprob is None else _ptr(logprob), _stream(logits))
+    _check(rc, "sample_tokens")
+    return (out, logprob) if return_logprobs else out

@@ -442,6 +442,47 @@ int ecc_decode_paged(const void *q_f16, const void *k_blocks, const void *v_bloc
                      int64_t ws_b, int64_t ws_h, void *workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
                      float sm_scale, int window, int sinks, int flags, ecc_stream_t stream);
 
+/* Cuts sequences of a paged cache down to `budget` tokens per kv head by
+ * accumulated attention weight, out of place: a sequence of L > budget tokens
+ * keeps its first `sinks`, its last `recent` and, of the others, the budget -
+ * sinks - recent with the largest weights (equal ones: the earlier; NaN above
+ * everything), in their order; a shorter one is kept whole.  Token i of the
+ * result goes to page out_pages->table[b][i / page_size] of the same pools;
+ * the new length is min(seq_lens[b], budget).
+ *   weights, out_weights: fp32, element (b, kv head, t) at b*s_b + h*s_h + t;
+ *     out_weights gets the kept tokens' weights and zeros up to out_len.
+ *   kept: int32 [B][Hkv][budget], positions that were kept, -1 behind them.
+ *   block_bytes: 128, or 96 for records.
+ *   workspace: ecc_evict_paged_workspace_size(n_pages) bytes.
+ * Pages that receive tokens must be distinct and hold none of the sequences'
+ * tokens: otherwise ecc_device_status 5, and no block is moved. */
+size_t ecc_evict_paged_workspace_size(int64_t n_pages);
+int ecc_evict_paged(void *k_blocks, void *v_blocks, int64_t bs_p, int64_t bs_h, const ecc_pages_t *pages,
+                    const int *seq_lens, const float *weights, int64_t ws_b, int64_t ws_h,
+                    const ecc_pages_t *out_pages, float *out_weights, int64_t ows_b, int64_t ows_h, int64_t out_len,
+                    int *kept, int B, int Hkv, int budget, int sinks, int recent, int block_bytes, void *workspace,
+                    size_t workspace_bytes, ecc_stream_t stream);
+
+/* ---- sampling -------------------------------------------------------------
+ * The next token of each of B rows of logits [B, V] (row_stride elements
+ * apart; dtype ECC_SAMPLE_*) from one given number in [0, 1) per row:
+ * temperature (0: the first maximum), then top-k (0: off), top-p (>= 1: off),
+ * min-p (0: off), each of which drops tokens; equal logits rank by ascending
+ * index.  Of what is kept, renormalised, the token is the first in ascending
+ * order at which the cumulative probability exceeds the number.  NaN counts as
+ * -inf; a row without a logit above -inf gives -1.  Each setting is one value
+ * for all rows or, when its pointer is not NULL, a DEVICE array [B].
+ *   token: int64 [B]; logprob: fp32 [B], log probability of the token among
+ *   the kept ones, or NULL.  1 <= V <= 2^20.  No counterpart in the reference,
+ *   whose generate() samples in Python. */
+#define ECC_SAMPLE_F16 0
+#define ECC_SAMPLE_BF16 1
+#define ECC_SAMPLE_F32 2
+int ecc_sample(const void *logits, int64_t row_stride, int dtype, int B, int64_t V, const float *uniform,
+               const float *temperature, float temperature_all, const int *top_k, int top_k_all, const float *top_p,
+               float top_p_all, const float *min_p, float min_p_all, int64_t *token, float *logprob,
+               ecc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
