@@ -18,22 +18,31 @@ namespace sel {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kCopies = 4;
 constexpr int kPerThread = kBins / kThreads;
 constexpr int kMaxCluster = 16;
 
+struct Crossing {  // see crossing()
+    uint32_t slot;
+    uint64_t before, here;
+};
+struct CrossingShared {
+    uint64_t share[kMaxCluster];  // the CTAs' sums of their bins, written by each of them
+    Crossing found;               // written by the CTA that finds it
+};
+
 struct alignas(16) Shared {
     uint32_t hist[kBins * kCopies];
     uint32_t sum[kBins];  // this CTA's counts of a pass, read by the cluster
+    uint32_t tot[kBins];  // the cluster's, this CTA's share of the bins
     uint32_t warp_a[kWarps], warp_b[kWarps];
     uint64_t warp64[kWarps];
     uint32_t cta_a, cta_b;  // totals of this CTA, read by the cluster
     uint64_t cta64;
-    uint32_t found[3];
-    uint64_t found64[2];
+    CrossingShared cross;
     uint32_t cut;  // written by the CTA that finds it
 };
 
@@ -61,15 +70,87 @@ __device__ __forceinline__ T block_exclusive(T v, T *warp_sums, T *total) {
     __syncthreads();  // earlier readers of warp_sums are done
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
-    T before = 0, all = 0;
+    // every warp adds up the warps' sums by itself: a scan over 32 lanes
+    static_assert(kWarps == 32, "a lane per warp");
+    const T w = warp_sums[lane];
+    T upto = w;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const T x = warp_sums[w];
-        before += w < warp ? x : 0;
-        all += x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const T x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
     }
+    const T before = __shfl_sync(0xffffffffu, upto - w, warp), all = __shfl_sync(0xffffffffu, upto, 31);
     *total = all;
     return before + inc - v;
+}
+
+// Sums over the cluster, spread over it: CTA r gets the sums of from[r W ..
+// r W + W), W = kBins / CTAs, in to[0 .. W).  All CTAs must have passed a
+// cluster barrier since their `from` was written, and pass one (crossing()
+// does) before it is written again.
+template <class T>
+__device__ __forceinline__ void cluster_share(cg::cluster_group &cl, T *from, T *to) {
+    const int ranks = (int)cl.num_blocks(), W = kBins / ranks, at = (int)cl.block_rank() * W;
+    for (int i = threadIdx.x; i < W; i += kThreads) {
+        T c = 0;
+        for (int r = 0; r < ranks; r += 8) {
+            T v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = r + q < ranks ? of_rank(cl, from, r + q)[at + i] : 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) c += v[q];
+        }
+        to[i] = c;
+    }
+    __syncthreads();
+}
+
+// The sum of all bins; every CTA's cs.share is filled.
+template <class T>
+__device__ __forceinline__ uint64_t share_sums(CrossingShared &cs, cg::cluster_group &cl, const T *bins,
+                                               uint64_t *warp_sums) {
+    const int ranks = (int)cl.num_blocks(), W = kBins / ranks;
+    uint64_t v = 0;
+    for (int i = threadIdx.x; i < W; i += kThreads) v += bins[i];
+    uint64_t mine;
+    block_exclusive(v, warp_sums, &mine);
+    if (threadIdx.x < ranks) of_rank(cl, cs.share, threadIdx.x)[cl.block_rank()] = mine;
+    cl.sync();
+    uint64_t all = 0;
+    for (int r = 0; r < ranks; ++r) all += cs.share[r];
+    return all;
+}
+// Where the running sum over the spread bins, whose share_sums() are known,
+// reaches `want` (1 <= want <= the sum of all): the bin, the sum before it and
+// its own, the same in every CTA.  Ends with a cluster barrier.
+template <class T>
+__device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_group &cl, const T *bins, uint64_t want,
+                                             uint64_t *warp_sums) {
+    const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), W = kBins / ranks;
+    uint64_t before = 0;
+    for (int r = 0; r < rank; ++r) before += cs.share[r];
+    const uint64_t mine = cs.share[rank];
+    if (before < want && want <= before + mine) {  // block-uniform
+        const int per = (W + kThreads - 1) / kThreads;
+        uint64_t v[kPerThread], sum = 0;
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            const int i = threadIdx.x * per + j;
+            v[j] = j < per && i < W ? bins[i] : 0;
+            sum += v[j];
+        }
+        uint64_t all;
+        before += block_exclusive(sum, warp_sums, &all);
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            if (before < want && want <= before + v[j])
+                for (int r = 0; r < ranks; ++r)
+                    of_rank(cl, &cs, r)->found = {(uint32_t)(rank * W + threadIdx.x * per + j), before, v[j]};
+            before += v[j];
+        }
+    }
+    cl.sync();
+    return cs.found;
 }
 
 // The k-th largest key of the cluster's row, 1 <= k <= keys of the row.
@@ -86,51 +167,39 @@ __device__ __forceinline__ uint32_t kth_largest(Shared &sh, cg::cluster_group &c
     while (top > low) {
         const int bits = min(11, top - low), shift = top - bits;
         const uint32_t bins = 1u << bits;
-        for (int i = tid; i < kBins * kCopies; i += kThreads) sh.hist[i] = 0;
+        for (int i = tid; i < kBins * kCopies / 4; i += kThreads)
+            reinterpret_cast<uint4 *>(sh.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
+#pragma unroll 4
         for (int i = tid; i < n; i += kThreads) {
             const uint32_t x = keys(i);
             if ((x & mask) == prefix) atomicAdd(&sh.hist[((x >> shift) & (bins - 1)) * kCopies + (tid & (kCopies - 1))], 1u);
         }
         __syncthreads();
-        for (int i = tid; i < kBins; i += kThreads)
-            sh.sum[i] = (sh.hist[4 * i] + sh.hist[4 * i + 1]) + (sh.hist[4 * i + 2] + sh.hist[4 * i + 3]);
+        // bins from the top, so that a prefix counts the larger keys
+        for (int i = tid; i < kBins; i += kThreads) {
+            const uint4 c = reinterpret_cast<const uint4 *>(sh.hist)[kBins - 1 - i];
+            sh.sum[i] = (c.x + c.y) + (c.z + c.w);
+        }
         cl.sync();
-        // thread t takes bins from the top: kBins - 1 - 4t and the three below
-        uint32_t c[kPerThread], mine = 0;
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            const int bin = kBins - 1 - (tid * kPerThread + j);
-            c[j] = 0;
-            for (unsigned r = 0; r < ranks; ++r) c[j] += of_rank(cl, sh.sum, r)[bin];
-            mine += c[j];
-        }
-        uint32_t all;
-        uint32_t before = block_exclusive(mine, sh.warp_a, &all);
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            if (before < k && k <= before + c[j]) {
-                sh.found[0] = kBins - 1 - (tid * kPerThread + j);
-                sh.found[1] = before;
-                sh.found[2] = c[j];
-            }
-            before += c[j];
-        }
-        cl.sync();  // found is written; every CTA has read the sums
-        prefix |= sh.found[0] << shift;
+        cluster_share(cl, sh.sum, sh.tot);
+        share_sums(sh.cross, cl, sh.tot, sh.warp64);
+        const Crossing f = crossing(sh.cross, cl, sh.tot, k, sh.warp64);
+        prefix |= (kBins - 1 - f.slot) << shift;
         mask |= (bins - 1) << shift;
-        k -= sh.found[1];
-        *equal = sh.found[2];
+        k -= (uint32_t)f.before;
+        *equal = (uint32_t)f.here;
         top = shift;
-        __syncthreads();
     }
     *ties = k;
     return prefix;
 }
 
-// A warp's contiguous part of the CTA's n elements.
+// A warp's contiguous part of the CTA's n elements, and the warp of element i.
+__device__ __forceinline__ int part_size(int n) { return ((n + kWarps - 1) / kWarps + 31) / 32 * 32; }
+__device__ __forceinline__ int part_of(int n, int i) { return i / part_size(n); }
 __device__ __forceinline__ void warp_part(int n, int &lo, int &hi) {
-    const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const int per = part_size(n);
     lo = min(n, (int)(threadIdx.x >> 5) * per);
     hi = min(n, lo + per);
 }
@@ -148,13 +217,8 @@ __device__ __forceinline__ uint32_t cluster_exclusive(Shared &sh, cg::cluster_gr
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = warp_value;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const uint32_t x = sh.warp_a[w];
-        before += w < warp ? x : 0;
-        all += x;
-    }
+    const uint32_t x = sh.warp_a[threadIdx.x & 31], all = __reduce_add_sync(0xffffffffu, x);
+    uint32_t before = __reduce_add_sync(0xffffffffu, (int)(threadIdx.x & 31) < warp ? x : 0);
     if (threadIdx.x == 0) sh.cta_a = all;
     cl.sync();
     for (unsigned r = 0; r < cl.block_rank(); ++r) before += *of_rank(cl, &sh.cta_a, r);
@@ -189,11 +253,11 @@ __device__ __forceinline__ uint32_t tie_cut(Shared &sh, cg::cluster_group &cl, i
     return cut;
 }
 
-// Cluster size for `rows` rows: the largest power of two up to `most` with
-// which every CTA still has an SM of its own.
-static inline int cluster_size(int64_t rows, int sms, int most) {
+// Cluster size for `rows` rows of `n` elements: the largest power of two up to
+// `most` with which every CTA still has an SM of its own and `least` elements.
+static inline int cluster_size(int64_t rows, int64_t n, int sms, int most, int least) {
     int c = 1;
-    while (c < most && rows * (2 * c) <= sms) c *= 2;
+    while (c < most && rows * (2 * c) <= sms && n >= (int64_t)least * 2 * c) c *= 2;
     return c;
 }
 

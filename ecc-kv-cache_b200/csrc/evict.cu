@@ -65,8 +65,9 @@ __device__ void check_tables(const EvictArgs &a, sel::cg::cluster_group &cl) {
 }
 
 __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __grid_constant__ EvictArgs a) {
-    extern __shared__ __align__(16) uint32_t cache[];
-    __shared__ sel::Shared sh;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    sel::Shared &sh = *reinterpret_cast<sel::Shared *>(dyn);
+    uint32_t *cache = reinterpret_cast<uint32_t *>(dyn + sizeof(sel::Shared));
     sel::cg::cluster_group cl = sel::cg::this_cluster();
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31;
     pdl_trigger();
@@ -248,11 +249,11 @@ extern "C" int ecc_evict_paged(void *k_blocks, void *v_blocks, int64_t bs_p, int
 
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int64_t rows = (int64_t)B * Hkv;
-    const int C = sel::cluster_size(rows, sm_count(), 8);
+    const int C = sel::cluster_size(rows, a.src.capacity, sm_count(), 8, 4096);
     // the keys of a slice stay in shared memory when they fit beside the counts
     const int64_t slice = (a.src.capacity + C - 1) / C;
-    a.cache_keys = (int)std::min<int64_t>(slice, 40000);
-    if (sel::launch_cluster(evict_select_kernel, C, rows + 1, (size_t)a.cache_keys * 4, s, a) != cudaSuccess)
+    a.cache_keys = (int)std::min<int64_t>(slice, (227 * 1024 - sizeof(sel::Shared)) / 4);
+    if (sel::launch_cluster(evict_select_kernel, C, rows + 1, sizeof(sel::Shared) + (size_t)a.cache_keys * 4, s, a) != cudaSuccess)
         return ECC_ERR_LAUNCH;
     rc = launch_status();
     if (rc != ECC_OK) return rc;

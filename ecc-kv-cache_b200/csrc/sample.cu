@@ -11,9 +11,11 @@
 //   logprob = log(w_token / total).  T = 0: the first maximum, logprob 0.
 //   A row without a logit above -inf: token -1, logprob -inf.
 //
-// No sort: one cluster of CTAs per row keeps the row in shared memory and
-// finds the thresholds by radix descents (cluster_select.cuh), first by count,
-// then by mass.  Masses are sums of fixed-point numbers w * 2^S (S = 62 -
+// No sort of the row: one cluster of CTAs per row keeps it in shared memory.
+// One pass bins the tokens by their distance from the maximum, with counts and
+// masses; the bin in which top-k or top-p ends is then sorted on its own (a
+// bin of too many equal logits is descended by key bits, cluster_select.cuh);
+// a last pass draws.  Masses are sums of fixed-point numbers w * 2^S (S = 62 -
 // ceil(log2 V), at least 42 bits behind the point), so they do not depend on
 // the order of the additions, and atomics give the same bits every time.
 // A drawn token hangs on which side of a sum u * total falls: fp32 exponentials
@@ -39,7 +41,6 @@ namespace samp {
 using namespace sel;
 
 constexpr int kTab = 512;
-constexpr int kMassBins = 2048;
 
 struct Args {
     const void *logits;
@@ -52,9 +53,8 @@ struct Args {
     int top_k0;
     int64_t *token;
     float *logprob;
-    int slice;    // elements of a row per CTA
-    bool cached;  // the slice is kept in shared memory
-    int S;        // fixed-point bits
+    int slice;  // elements of a row per CTA
+    int S;      // fixed-point bits
 };
 
 template <class T>
@@ -80,13 +80,46 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~(k | ~(0xffffffffu << key_low<T>())));
 }
 
-struct Extra {
+struct Work {
+    Shared sel;
+    unsigned long long tot_mass[kBins];  // the cluster's masses and counts, this CTA's share of the bins
+    uint32_t tot_count[kBins];
     double tab[kTab];
     float best;
     uint32_t best_at;
     float cta_best;       // of this CTA, read by the cluster
     uint32_t cta_best_at;
+    uint32_t listed;      // rank 0: entries of the list
+    uint32_t kth, cut;    // written by rank 0
+    uint64_t bin_mass;
+    unsigned long long part[kWarps];
+    int lo, hi;           // the part that holds the drawn token, and the mass before it
+    uint64_t before;
 };
+// In the place of the count descent's bins: this CTA's counts and masses of
+// the first pass, later (rank 0) the list of one bin's tokens.
+struct Bins {
+    uint32_t count[kBins];
+    unsigned long long mass[kBins];
+};
+constexpr int kList = sizeof(Shared::hist) / 8;
+static_assert(sizeof(Bins) <= sizeof(Shared::hist), "room for the bins");
+
+// Descending sort of the first power of two >= n entries (those from n on must
+// be zero) of `x` by the whole block.
+__device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
+    int size = 1;
+    while (size < n) size *= 2;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+                const int i = 2 * t - (t & (j - 1));  // bit j of i is clear
+                const unsigned long long p = x[i], q = x[i + j];
+                if ((p < q) == ((i & k) == 0)) x[i] = q, x[i + j] = p;
+            }
+            __syncthreads();
+        }
+}
 
 // w * 2^S as an integer.
 struct Mass {
@@ -95,15 +128,15 @@ struct Mass {
     int S;
     __device__ __forceinline__ uint64_t operator()(float x) const {
         if (x == (float)best) return 1ull << S;
-        const double z = ((double)x - best) * inv_t;
-        if (!(z > -44.0)) return 0;  // below 2^-63, and -inf
+        const double d = (double)x - best;
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
-        const double t = fma(z, kTab / 0.693147180559945309417, kMagic);
+        const double t = fma(d, inv_t * (kTab / 0.693147180559945309417), kMagic);
+        if (!(t > kMagic - 44.0 * 740.0)) return 0;  // w below 2^-63, and x = -inf
         const int n = __double2loint(t);
-        const double m = t - kMagic;
-        const double r = fma(m, -0.693147180559945309417 / kTab, z);  // |m ln2/512| < 44: off by 2^-47 at most
+        // r = d / T - n ln2 / 512, |n ln2 / 512| < 45: off by 2^-47 at most
+        const double r = fma(d, inv_t, (t - kMagic) * (-0.693147180559945309417 / kTab));
         const double p = fma(r, fma(r, fma(r, 1.0 / 6.0, 0.5), 1.0), 1.0);
-        const double w = p * tab[n & (kTab - 1)];
+        const double w = p * tab[n & (kTab - 1)];  // 1 <= w < 2.002
         // 2^S * 2^(n div 512) enters through the exponent; the rounding to an integer by adding 2^52
         const double scaled = __hiloint2double(__double2hiint(w) + ((S + (n >> 9)) << 20), __double2loint(w));
         return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
@@ -128,43 +161,96 @@ __device__ __forceinline__ uint64_t share_of(float f, uint64_t total, bool *cut_
     return hi >> (s - 64);
 }
 
-template <class T>
+// Sum of v over the cluster's threads.
+__device__ __forceinline__ uint64_t cluster_sum(Shared &sh, cg::cluster_group &cl, uint64_t v) {
+    uint64_t all;
+    block_exclusive(v, sh.warp64, &all);
+    if (threadIdx.x == 0) sh.cta64 = all;
+    cl.sync();
+    all = 0;
+    for (unsigned r = 0; r < cl.num_blocks(); ++r) all += *of_rank(cl, &sh.cta64, r);
+    cl.sync();
+    return all;
+}
+
+// The top-p threshold inside a bin of many (nearly) equal logits, by the bits
+// of their keys: a descent like kth_largest's whose digits are found by mass.
+// Returns the new threshold key and cut.
+template <class T, class Load, class Keep, class BinOf>
+__device__ __noinline__ uint2 mass_descent(Shared &sh, Load load, Keep keep, BinOf bin_of, Mass mass, int n, int base,
+                                           int bin, uint64_t above, uint64_t want, uint32_t kth, uint32_t cut) {
+    cg::cluster_group cl = cg::this_cluster();
+    unsigned long long *from = reinterpret_cast<unsigned long long *>(sh.hist), *to = from + kBins;
+    const int tid = threadIdx.x, low = key_low<T>();
+    uint32_t prefix = 0, mask = 0;
+    uint64_t at = 0;
+    for (int top = 32; top > low;) {
+        const int bits = min(11, top - low), shift = top - bits;
+        for (int i = tid; i < kBins; i += kThreads) from[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            const float x = load(i);
+            const uint32_t kx = value_key<T>(x);
+            if ((kx & mask) != prefix || !keep(kx, i) || bin_of(x) != bin) continue;
+            const uint64_t w = mass(x);
+            if (w) atomicAdd(&from[kBins - 1 - ((kx >> shift) & ((1u << bits) - 1))], (unsigned long long)w);
+        }
+        cl.sync();
+        cluster_share(cl, from, to);
+        share_sums(sh.cross, cl, to, sh.warp64);
+        const Crossing f = crossing(sh.cross, cl, to, want - above, sh.warp64);
+        above += f.before;
+        at = f.here;
+        prefix |= (kBins - 1 - f.slot) << shift;
+        mask |= ((1u << bits) - 1) << shift;
+        top = shift;
+    }
+    // every kept token with this key has the same mass: the smallest m with above + m w >= want > above
+    const uint64_t w = max((uint64_t)1, mass(key_value<T>(prefix)));
+    const uint64_t m = (want - above + w - 1) / w, count = at / w;
+    uint32_t new_cut = prefix == kth ? cut : 0xffffffffu;
+    if (m < count)
+        new_cut = tie_cut(sh, cl, n, base, (uint32_t)m, [&](int i) {
+            const uint32_t kx = value_key<T>(load(i));
+            return kx == prefix && keep(kx, i);
+        });
+    return make_uint2(prefix, new_cut);
+}
+
+template <class T, bool kCached>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t dyn[];
-    __shared__ Shared sh;
-    __shared__ Extra ex;
-    // masses by bin, read by the cluster: in the place of a count descent's bins
-    unsigned long long *mass_bins = reinterpret_cast<unsigned long long *>(sh.hist);
-    static_assert(sizeof(sh.hist) >= kMassBins * 8, "room for the masses");
+    Work &wk = *reinterpret_cast<Work *>(dyn);
+    Shared &sh = wk.sel;
+    T *x_s = reinterpret_cast<T *>(dyn + (sizeof(Work) + 15) / 16 * 16);
     cg::cluster_group cl = cg::this_cluster();
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / C;
-    for (int i = tid; i < kTab; i += kThreads) ex.tab[i] = exp2((double)i / kTab);
+    for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab);
+    if (tid == 0) wk.listed = 0;
     pdl_trigger();
     pdl_wait();
 
-    const T *x_row = reinterpret_cast<const T *>(a.logits) + (int64_t)row * a.row_stride;
     const int base = min(a.V, rank * a.slice), n = min(a.V, base + a.slice) - base;
-    const T *x_g = x_row + base;
-    T *x_s = reinterpret_cast<T *>(dyn);
-    const bool cached = a.cached;
-    auto load = [&](int i) {
-        const float x = to_float<T>(cached ? x_s[i] : x_g[i]);
+    const T *x_g = reinterpret_cast<const T *>(a.logits) + (int64_t)row * a.row_stride + base;
+    auto load = [x_s, x_g](int i) {
+        const float x = to_float<T>(kCached ? x_s[i] : x_g[i]);
         return x != x ? -INFINITY : x;
     };
 
     // ---- the row, its maximum and the maximum's first place
     float best = -INFINITY;
     uint32_t best_at = 0xffffffffu;
-    if (cached) {
+    if (kCached) {
         constexpr int kVec = 16 / sizeof(T);
-        const bool wide = ((uintptr_t)x_g & 15) == 0;
-        const int n_wide = wide ? n / kVec : 0;
+        const int n_wide = ((uintptr_t)x_g & 15) == 0 ? n / kVec : 0;
+#pragma unroll 4
         for (int i = tid; i < n_wide; i += kThreads)
             reinterpret_cast<uint4 *>(x_s)[i] = __ldg(reinterpret_cast<const uint4 *>(x_g) + i);
         for (int i = n_wide * kVec + tid; i < n; i += kThreads) x_s[i] = x_g[i];
         __syncthreads();
     }
+#pragma unroll 4
     for (int i = tid; i < n; i += kThreads) {
         const float x = load(i);
         if (x > best) best = x, best_at = base + i;  // ascending i: the first of equals
@@ -172,25 +258,29 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     auto better = [](float x, uint32_t i, float &bx, uint32_t &bi) {
         if (x > bx || (x == bx && i < bi)) bx = x, bi = i;
     };
+    auto warp_best = [&]() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o), best, best_at);
+        for (int o = 16; o > 0; o >>= 1)
+            better(__shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_at, o), best, best_at);
+    };
+    warp_best();
     if (lane == 0) sh.warp_a[warp] = __float_as_uint(best), sh.warp_b[warp] = best_at;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) better(__uint_as_float(sh.warp_a[w]), sh.warp_b[w], best, best_at);
-        ex.cta_best = best;
-        ex.cta_best_at = best_at;
+    if (warp == 0) {
+        best = __uint_as_float(sh.warp_a[lane]), best_at = sh.warp_b[lane];
+        warp_best();
+        if (lane == 0) wk.cta_best = best, wk.cta_best_at = best_at;
     }
     cl.sync();
-    if (tid == 0) {
-        for (int r = 0; r < C; ++r) better(*of_rank(cl, &ex.cta_best, r), *of_rank(cl, &ex.cta_best_at, r), best, best_at);
-        ex.best = best;
-        ex.best_at = best_at;
+    if (warp == 0) {
+        best = -INFINITY, best_at = 0xffffffffu;
+        if (lane < C) best = *of_rank(cl, &wk.cta_best, lane), best_at = *of_rank(cl, &wk.cta_best_at, lane);
+        warp_best();
+        if (lane == 0) wk.best = best, wk.best_at = best_at;
     }
     cl.sync();  // also: nobody reads a CTA's shared memory after it may have left
-    best = ex.best;
-    best_at = ex.best_at;
+    best = wk.best;
+    best_at = wk.best_at;
     const float temp = a.temperature ? __ldg(a.temperature + row) : a.temperature0;
     if (best == -INFINITY || !(temp > 0.0f)) {  // cluster-uniform
         if (rank == 0 && tid == 0) {
@@ -199,176 +289,423 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         }
         return;
     }
-    const Mass mass{ex.tab, (double)best, 1.0 / (double)temp, a.S};
+    const Mass mass{wk.tab, (double)best, 1.0 / (double)temp, a.S};
 
-    // ---- top-k: keys above `kth` are kept, equal ones below the row position `cut`
+    // What is kept so far: keys above `kth`, equal ones below the row position `cut`.
     uint32_t kth = 0, cut = 0xffffffffu;
     auto key = [&](int i) { return value_key<T>(load(i)); };
-    const int k = a.top_k ? __ldg(a.top_k + row) : a.top_k0;
-    if (k > 0 && k < a.V) {
-        uint32_t ties, equal;
-        kth = kth_largest(sh, cl, key, n, (uint32_t)k, key_low<T>(), &ties, &equal);
-        if (ties < equal) cut = tie_cut(sh, cl, n, base, ties, [&](int i) { return key(i) == kth; });
-    }
     auto keep = [&](uint32_t x, int i) { return x > kth || (x == kth && (uint32_t)(base + i) < cut); };
 
-    // ---- top-p
+    const int k = a.top_k ? __ldg(a.top_k + row) : a.top_k0;
     const float p = a.top_p ? __ldg(a.top_p + row) : a.top_p0;
-    if (p < 1.0f) {
-        // First by the distance from the maximum in bins of 1/64 (monotone in x, and spread however the
-        // logits lie), then by the bits of the key among those of the bin that holds the threshold.
+    const bool by_count = k > 0 && k < a.V, by_mass = p < 1.0f;
+    const float mp = a.min_p ? __ldg(a.min_p + row) : a.min_p0;
+    // w >= min_p as whole masses; the most likely token stays in any case
+    const uint64_t least = mp > 0.0f ? (uint64_t)ceil(fmin((double)mp, 1.0) * (double)(1ull << a.S)) : 0;
+    const float u = __ldg(a.u + row);
+    // cumulative mass > u * total, of whole masses: > floor(u * total); a number of 1 or more takes the last
+    // kept token, one that is not above 0 the first
+    auto need_of = [u](uint64_t total) -> uint64_t {
+        bool ignored;
+        return !(u > 0.0f) ? 0 : u < 1.0f ? share_of(u, total, &ignored) : total - 1;
+    };
+    // ceil(p * total): whole sums below it are below p * total.  p <= 0: the first token alone.
+    auto want_of = [p](uint64_t total) {
+        bool more = true;
+        const uint64_t want = p > 0.0f ? share_of(p, total, &more) : 0;
+        return want + (more ? 1 : 0);
+    };
+
+    bool parts_known = false;  // wk.part holds the kept masses of the warps' parts
+    if (by_count || by_mass) {
+        // ---- counts and masses by the distance from the maximum, in bins of 1/64 of an e-fold: monotone in
+        // x, and spread however the logits lie
+        Bins &bins = *reinterpret_cast<Bins *>(sh.hist);
+        unsigned long long *list = reinterpret_cast<unsigned long long *>(sh.hist);
         const float inv_bin = 64.0f / temp;
-        auto bin_of = [&](float x) {
-            const float d = (best - x) * inv_bin;  // NaN when x is the infinite maximum
-            return x == best ? 0 : d < (float)(kMassBins - 1) ? (int)d : kMassBins - 1;
+        auto distance = [best, inv_bin](float x) {  // in bins; not of the infinite maximum itself
+            return x == best ? 0.0f : (best - x) * inv_bin;
         };
-        int bin = -1;
-        uint32_t prefix = 0, mask = 0;
-        uint64_t above = 0, at = 0;  // mass above the bin, of the bin
-        uint64_t want = 0;           // ceil(p * total): whole masses below it are below p * total
-        int top = 33;
-        while (true) {
-            const int low = key_low<T>(), bits = top == 33 ? 11 : min(11, top - low), shift = top - bits;
-            for (int i = tid; i < kMassBins; i += kThreads) mass_bins[i] = 0;
+        auto bin_of = [distance](float x) {
+            const float d = distance(x);
+            return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+        };
+        // What a pass adds up per bin: counts, and with them nothing, the places inside the bin (a sum of
+        // kPlaces-ths of its width), or the masses.
+        constexpr int kCount = 0, kPlace = 1, kMassToo = 2;
+        constexpr float kPlaces = 1024.0f;
+        auto count_bins = [&](auto what) {
+            constexpr bool kMass = decltype(what)::value == kMassToo, kPlaced = decltype(what)::value == kPlace;
+            for (int i = tid; i < kBins; i += kThreads) {
+                bins.count[i] = 0;
+                if (kMass || kPlaced) bins.mass[i] = 0;
+            }
             __syncthreads();
+            // everything far below goes to the last bin: added up per thread first
+            uint32_t far_count = 0;
+            uint64_t far_mass = 0;
+#pragma unroll 4
             for (int i = tid; i < n; i += kThreads) {
-                const float x = load(i);
-                const uint32_t kx = value_key<T>(x);
-                if (!keep(kx, i)) continue;
-                const int mine = bin_of(x);
-                // bin 0 of the mass array is the top one in either kind of pass
-                int slot;
-                if (bin < 0) {
-                    slot = mine;
+                const float x = load(i), d = distance(x);
+                const uint64_t w = kMass ? mass(x) : 0;
+                if (!(d < (float)(kBins - 1))) {
+                    ++far_count;
+                    far_mass += w;
                 } else {
-                    if (mine != bin || (kx & mask) != prefix) continue;
-                    slot = kMassBins - 1 - (int)((kx >> shift) & ((1u << bits) - 1));
+                    const int b = (int)d;
+                    atomicAdd(&bins.count[b], 1u);
+                    if (kMass) atomicAdd(&bins.mass[b], (unsigned long long)w);
+                    // the low half of the bin's 64 bits: at most 2^20 tokens, fewer than 2^10 places each
+                    if (kPlaced)
+                        atomicAdd(reinterpret_cast<uint32_t *>(&bins.mass[b]), (uint32_t)((d - (float)b) * kPlaces));
                 }
-                const uint64_t w = mass(x);
-                if (w) atomicAdd(&mass_bins[slot], (unsigned long long)w);
+            }
+            far_count = __reduce_add_sync(0xffffffffu, far_count);
+            if (kMass) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) far_mass += __shfl_xor_sync(0xffffffffu, far_mass, o);
+            }
+            if (lane == 0 && far_count) {
+                atomicAdd(&bins.count[kBins - 1], far_count);
+                if (kMass) atomicAdd(&bins.mass[kBins - 1], (unsigned long long)far_mass);
             }
             cl.sync();
-            uint64_t c[kPerThread], mine = 0;
-#pragma unroll
-            for (int j = 0; j < kPerThread; ++j) {
-                c[j] = 0;
-                for (int r = 0; r < C; ++r) c[j] += of_rank(cl, mass_bins, r)[tid * kPerThread + j];
-                mine += c[j];
-            }
-            uint64_t all;
-            uint64_t before = block_exclusive(mine, sh.warp64, &all);
-            if (bin < 0) {
-                bool more = true;
-                want = p > 0.0f ? share_of(p, all, &more) : 0;  // p <= 0: the first token alone
-                want += more ? 1 : 0;
-            }
-            before += above;
-#pragma unroll
-            for (int j = 0; j < kPerThread; ++j) {
-                // the bin before which less than the wanted mass lies, and after which not
-                if (before < want && want <= before + c[j]) {
-                    sh.found[0] = tid * kPerThread + j;
-                    sh.found64[0] = before;
-                    sh.found64[1] = c[j];
-                }
-                before += c[j];
-            }
+            cluster_share(cl, bins.count, wk.tot_count);
+            if (kMass || kPlaced) cluster_share(cl, bins.mass, wk.tot_mass);
+            share_sums(sh.cross, cl, wk.tot_count, sh.warp64);  // its barrier: the bins' place is free
+        };
+        // Puts the kept ones of a warp's elements into rank 0's list (room for kList) as (key, ~row position).
+        auto append = [&](bool hit, int i) {
+            const uint32_t kx = hit ? value_key<T>(load(i)) : 0;
+            hit = hit && keep(kx, i);
+            const uint32_t m = __ballot_sync(0xffffffffu, hit);
+            if (!m) return;
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(of_rank(cl, &wk.listed, 0), (uint32_t)__popc(m));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
+            if (hit) of_rank(cl, list, 0)[at] = ((unsigned long long)kx << 32) | (uint32_t)~(uint32_t)(base + i);
+        };
+        // Waits for the list and sorts it in rank 0, descending.  Returns its length.
+        auto sorted = [&]() {
             cl.sync();
-            above = sh.found64[0];
-            at = sh.found64[1];
-            if (bin < 0) {
-                bin = sh.found[0];
-                top = 32;
-            } else {
-                prefix |= (uint32_t)(kMassBins - 1 - sh.found[0]) << shift;
-                mask |= ((1u << bits) - 1) << shift;
-                top = shift;
+            const int m = wk.listed;
+            if (rank == 0) {
+                int size = 1;
+                while (size < m) size *= 2;
+                for (int i = m + tid; i < size; i += kThreads) list[i] = 0;
+                __syncthreads();
+                sort_descending(list, m);
+            }
+            return m;
+        };
+        // The kept tokens of bins b0 .. b1 in the list, sorted.
+        auto gather = [&](int b0, int b1) {
+            const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
+            constexpr int kTake = 4;
+            for (int i0 = warp * 32; i0 < n; i0 += kThreads * kTake) {
+                bool hit[kTake], any = false;
+#pragma unroll
+                for (int q = 0; q < kTake; ++q) {
+                    const int i = i0 + q * kThreads + lane;
+                    const float d = i < n ? distance(load(i)) : -1.0f;
+                    hit[q] = !(d < d0) && !(d >= d1);
+                    any = any || hit[q];
+                }
+                if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+                for (int q = 0; q < kTake; ++q) append(hit[q], i0 + q * kThreads + lane);
+            }
+            return sorted();
+        };
+        auto listed_mass = [&](int i) { return mass(key_value<T>((uint32_t)(list[i] >> 32))); };
+        // Rank 0's finding reaches the cluster; the list is free again.
+        auto publish = [&](unsigned long long entry) {
+            for (int r = 0; r < C; ++r)
+                *of_rank(cl, &wk.kth, r) = (uint32_t)(entry >> 32), *of_rank(cl, &wk.cut, r) = ~(uint32_t)entry + 1;
+        };
+        auto take = [&]() {
+            cl.sync();
+            kth = wk.kth;
+            cut = wk.cut;
+            if (tid == 0) wk.listed = 0;
+            cl.sync();
+        };
+
+        Crossing at_k{};
+        if (by_count) {
+            count_bins(std::integral_constant<int, kCount>());
+            at_k = crossing(sh.cross, cl, wk.tot_count, (uint64_t)k, sh.warp64);
+            if (at_k.before + at_k.here <= kList) {
+                // everything that may be kept fits the list: rank 0 finishes alone
+                gather(0, (int)at_k.slot);
+                if (rank != 0) return;  // nobody reads the other CTAs' shared memory any more
+                int kept = k;
+                if (by_mass || least > 0) {
+                    uint64_t sum = 0, want = 0, total;
+                    if (by_mass) {
+                        for (int i = tid; i < kept; i += kThreads) sum += listed_mass(i);
+                        block_exclusive(sum, sh.warp64, &total);
+                        want = want_of(total);
+                    }
+                    uint64_t before = 0;
+                    uint32_t stay = 0;
+                    for (int i0 = 0; i0 < kept; i0 += kThreads) {  // block-uniform
+                        const int i = i0 + tid;
+                        const uint64_t w = i < kept ? listed_mass(i) : 0;
+                        uint64_t all;
+                        const uint64_t mine = before + block_exclusive(w, sh.warp64, &all);
+                        // both conditions hold for a first part of the list
+                        stay += i < kept && (i == 0 || ((!by_mass || mine < want) && w >= least)) ? 1 : 0;
+                        before += all;
+                    }
+                    uint32_t all;
+                    block_exclusive(stay, sh.warp_a, &all);
+                    kept = (int)all;
+                }
+                // by row position, and the draw
+                for (int i = tid; i < kept; i += kThreads) list[i] = (list[i] << 32) | (list[i] >> 32);
+                int size = 1;
+                while (size < kept) size *= 2;
+                for (int i = kept + tid; i < size; i += kThreads) list[i] = 0;
+                __syncthreads();
+                sort_descending(list, kept);
+                auto drawn_mass = [&](int i) { return mass(key_value<T>((uint32_t)list[i])); };
+                uint64_t sum = 0, total;
+                for (int i = tid; i < kept; i += kThreads) sum += drawn_mass(i);
+                block_exclusive(sum, sh.warp64, &total);
+                const uint64_t need = need_of(total);
+                uint64_t before = 0;
+                for (int i0 = 0; i0 < kept; i0 += kThreads) {
+                    const int i = i0 + tid;
+                    const uint64_t w = i < kept ? drawn_mass(i) : 0;
+                    uint64_t all;
+                    const uint64_t mine = before + block_exclusive(w, sh.warp64, &all);
+                    if (mine <= need && need < mine + w) {
+                        a.token[row] = (uint32_t)~(uint32_t)(list[i] >> 32);
+                        if (a.logprob) a.logprob[row] = (float)log((double)w / (double)total);
+                    }
+                    before += all;
+                }
+                return;
+            }
+        }
+        if (by_mass && !by_count) {
+            // ---- top-p alone: the bins' masses from counts and places tell where it ends, to 10^-4 of the mass;
+            // one pass over exact masses then adds up what surely stays and lists what lies near the end.
+            count_bins(std::integral_constant<int, kPlace>());
+            const int W = kBins / C;
+            for (int i = tid; i < W; i += kThreads) {
+                // e^(-f/64), 0 <= f < 1, as its chord less half its sag: off by 1.6e-5.  A place is off by half
+                // of 1/1024 of a bin: 8e-6.  fp32 here: 2e-7.  Everything in the last bin weighs at most e^-32.
+                const float n_b = (float)wk.tot_count[i];
+                const float f = ((float)(uint32_t)wk.tot_mass[i] + 0.5f * n_b) * (1.0f / kPlaces);
+                constexpr float kChord = 0.015503561f;  // 1 - e^(-1/64)
+                const float m = expf(-(float)(rank * W + i) * (1.0f / 64.0f)) * (n_b * (1.0f - 1.52e-5f) - kChord * f);
+                wk.tot_mass[i] = (unsigned long long)((double)fmaxf(m, 0.0f) * (double)(1ull << a.S));
             }
             __syncthreads();
-            if (top <= low) break;
+            const uint64_t about = share_sums(sh.cross, cl, wk.tot_mass, sh.warp64);
+            const uint64_t slack = about / 8192, aim = want_of(about);
+            const Crossing from = crossing(sh.cross, cl, wk.tot_mass, aim > slack ? aim - slack : 1, sh.warp64);
+            cl.sync();  // every CTA has its copy; the second search starts from the same sums
+            const Crossing to = crossing(sh.cross, cl, wk.tot_mass, min(aim + slack, about), sh.warp64);
+            const int b0 = (int)from.slot, b1 = aim + slack < about ? (int)to.slot : kBins - 1;
+            // tokens in b0 .. b1
+            uint32_t near = 0;
+            for (int i = tid; i < W; i += kThreads)
+                near += rank * W + i >= b0 && rank * W + i <= b1 ? wk.tot_count[i] : 0;
+            if (cluster_sum(sh, cl, near) <= kList) {
+                const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
+                int lo, hi;
+                warp_part(n, lo, hi);
+                uint64_t all = 0, above = 0, part = 0;
+                constexpr int kTake = 4;
+                for (int i0 = lo; i0 < hi; i0 += 32 * kTake) {
+                    bool hit[kTake], any = false;
+#pragma unroll
+                    for (int q = 0; q < kTake; ++q) {
+                        const int i = i0 + 32 * q + lane;
+                        hit[q] = false;
+                        if (i < hi) {
+                            const float x = load(i), d = distance(x);
+                            const uint64_t w = mass(x);
+                            const bool in = d < d0;
+                            all += w;
+                            above += in ? w : 0;
+                            part += in && w >= least ? w : 0;
+                            hit[q] = !in && !(d >= d1);
+                            any = any || hit[q];
+                        }
+                    }
+                    if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+                    for (int q = 0; q < kTake; ++q) append(hit[q], i0 + 32 * q + lane);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+                if (lane == 0) wk.part[warp] = part;
+                const uint64_t want = want_of(cluster_sum(sh, cl, all));
+                above = cluster_sum(sh, cl, above);
+                const int m = sorted();
+                if (rank == 0) {
+                    if (tid == 0) for (int r = 0; r < C; ++r) *of_rank(cl, &wk.kth, r) = 0;
+                    __syncthreads();
+                    // the part of a row position: its CTA's slice, its warp's share of the slice
+                    uint64_t before = above;
+                    for (int i0 = 0; i0 < m; i0 += kThreads) {  // block-uniform
+                        const int i = i0 + tid;
+                        const uint64_t w = i < m ? listed_mass(i) : 0;
+                        uint64_t sum;
+                        const uint64_t mine = before + block_exclusive(w, sh.warp64, &sum);
+                        if (i < m && mine < want) {
+                            if (want <= mine + w) publish(list[i]);
+                            if (w >= least) {
+                                const int at = (int)~(uint32_t)list[i], r = at / a.slice;
+                                atomicAdd(of_rank(cl, wk.part, r) + part_of(min(a.slice, a.V - r * a.slice), at - r * a.slice),
+                                          (unsigned long long)w);
+                            }
+                        }
+                        before += sum;
+                    }
+                }
+                take();
+                parts_known = kth != 0;  // no key is 0
+                if (!parts_known) cut = 0xffffffffu;  // the end was not in the list: the exact search below
+            }
         }
-        // every kept token with the threshold's key has the same mass
-        const uint32_t key_p = prefix;
-        const uint64_t w = max((uint64_t)1, mass(key_value<T>(key_p)));
-        const uint64_t count = at / w;
-        // how many of them: the smallest m with above + m w >= want > above
-        const uint64_t m = (want - above + w - 1) / w;
-        uint32_t cut_p = key_p == kth ? cut : 0xffffffffu;
-        if (m < count) {
-            const uint32_t old = cut_p;
-            cut_p = tie_cut(sh, cl, n, base, (uint32_t)m,
-                            [&](int i) { return key(i) == key_p && (uint32_t)(base + i) < old; });
+        if (by_mass && !parts_known) count_bins(std::integral_constant<int, kMassToo>());
+        if (by_count) {
+            const int b = (int)at_k.slot;
+            const uint32_t rest = (uint32_t)k - (uint32_t)at_k.before;
+            uint64_t dropped = 0;
+            if (at_k.here <= kList) {
+                const int m = gather(b, b);
+                if (rank == 0) {
+                    if (tid == 0) publish(list[rest - 1]);
+                    uint64_t mine = 0;
+                    if (by_mass)
+                        for (int i = rest + tid; i < m; i += kThreads) mine += listed_mass(i);
+                    block_exclusive(mine, sh.warp64, &dropped);
+                    if (tid < C) *of_rank(cl, &wk.bin_mass, tid) = dropped;
+                }
+                take();
+                dropped = wk.bin_mass;
+            } else {
+                // a bin with more equal or nearly equal logits than the list holds
+                uint32_t ties, equal;
+                const uint32_t x = kth_largest(sh, cl, key, n, (uint32_t)k, key_low<T>(), &ties, &equal);
+                if (ties < equal) cut = tie_cut(sh, cl, n, base, ties, [&](int i) { return key(i) == x; });
+                kth = x;
+                if (by_mass) {
+                    uint64_t mine = 0;
+                    for (int i = tid; i < n; i += kThreads)
+                        if (bin_of(load(i)) == b && !keep(key(i), i)) mine += mass(load(i));
+                    dropped = cluster_sum(sh, cl, mine);
+                }
+            }
+            if (by_mass) {
+                // the masses of what is left: the bins below are empty, this one has lost `dropped`
+                const int W = kBins / C;
+                for (int i = tid; i < W; i += kThreads) {
+                    if (rank * W + i > b) wk.tot_mass[i] = 0;
+                    if (rank * W + i == b) wk.tot_mass[i] -= dropped;
+                }
+                __syncthreads();
+            }
         }
-        kth = key_p;
-        cut = cut_p;
+        if (by_mass && !parts_known) {
+            const uint64_t want = want_of(share_sums(sh.cross, cl, wk.tot_mass, sh.warp64));
+            const Crossing at = crossing(sh.cross, cl, wk.tot_mass, want, sh.warp64);
+            const int b = (int)at.slot, W = kBins / C;
+            if (*of_rank(cl, wk.tot_count + b % W, b / W) <= kList) {
+                const int m = gather(b, b);
+                if (rank == 0) {
+                    uint64_t before = at.before;
+                    for (int i0 = 0; i0 < m; i0 += kThreads) {  // block-uniform
+                        const int i = i0 + tid;
+                        const uint64_t w = i < m ? listed_mass(i) : 0;
+                        uint64_t all;
+                        const uint64_t mine = before + block_exclusive(w, sh.warp64, &all);
+                        if (mine < want && want <= mine + w) publish(list[i]);
+                        before += all;
+                    }
+                }
+                take();
+            } else {
+                const auto kept = [kth, cut, base](uint32_t x, int i) {
+                    return x > kth || (x == kth && (uint32_t)(base + i) < cut);
+                };
+                const uint2 found = mass_descent<T>(sh, load, kept, bin_of, mass, n, base, b, at.before, want, kth, cut);
+                kth = found.x;
+                cut = found.y;
+            }
+        }
     }
 
     // ---- the draw: masses of the warps' parts, then the part that holds the number
-    const float mp = a.min_p ? __ldg(a.min_p + row) : a.min_p0;
-    const double least = (double)mp * (double)(1ull << a.S);
     auto kept_mass = [&](int i) -> uint64_t {
         const float x = load(i);
         if (!keep(value_key<T>(x), i)) return 0;
         const uint64_t w = mass(x);
-        return (double)w >= least || x == best ? w : 0;
+        return w >= least ? w : 0;
     };
     int lo, hi;
     warp_part(n, lo, hi);
     uint64_t part = 0;
-    for (int i = lo + lane; i < hi; i += 32) part += kept_mass(i);
+    if (parts_known) {
+        part = wk.part[warp];
+    } else {
+#pragma unroll 4
+        for (int i = lo + lane; i < hi; i += 32) part += kept_mass(i);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    }
     uint64_t cta_all;
     uint64_t before = block_exclusive(lane == 0 ? part : 0, sh.warp64, &cta_all);
     before = __shfl_sync(0xffffffffu, before, 0);
-    if (tid == 0) sh.cta64 = cta_all;
-    cl.sync();
-    uint64_t total = 0;
+    if (tid < C) of_rank(cl, sh.cross.share, tid)[rank] = cta_all;
+    cl.sync();  // nobody reads or writes another CTA's shared memory after this
+    uint64_t total = 0, cta_before = 0;
     for (int r = 0; r < C; ++r) {
-        const uint64_t c = *of_rank(cl, &sh.cta64, r);
-        before += r < rank ? c : 0;
-        total += c;
+        cta_before += r < rank ? sh.cross.share[r] : 0;
+        total += sh.cross.share[r];
     }
-    cl.sync();  // no remote reads after this
-    // cumulative mass > u * total, of whole masses: > floor(u * total); a number of 1 or more takes the last
-    // kept token, one that is not above 0 the first
-    const float u = __ldg(a.u + row);
-    bool ignored;
-    const uint64_t need = !(u > 0.0f) ? 0 : u < 1.0f ? share_of(u, total, &ignored) : total - 1;
-    if (part && before <= need && need < before + part) {  // this warp holds it
-        uint64_t seen = before;
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const uint64_t w = i0 + lane < hi ? kept_mass(i0 + lane) : 0;
-            uint64_t inc = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, seen + inc > need);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    a.token[row] = base + i0 + lane;
-                    if (a.logprob) a.logprob[row] = (float)log((double)w / (double)total);
-                }
-                break;
-            }
-            seen += __shfl_sync(0xffffffffu, inc, 31);
+    const uint64_t need = need_of(total);
+    if (need < cta_before || need >= cta_before + cta_all) return;  // block-uniform
+    before += cta_before;
+    if (lane == 0 && before <= need && need < before + part) wk.lo = lo, wk.hi = hi, wk.before = before;
+    __syncthreads();
+    // the part's elements over the block, a run of neighbours per thread
+    lo = wk.lo;
+    hi = wk.hi;
+    const int run = (hi - lo + kThreads - 1) / kThreads;
+    const int i0 = lo + tid * run, i1 = min(hi, i0 + run);
+    uint64_t mine = 0;
+    for (int i = i0; i < i1; ++i) mine += kept_mass(i);
+    uint64_t ignored;
+    before = wk.before + block_exclusive(mine, sh.warp64, &ignored);
+    if (need < before || need >= before + mine) return;
+    for (int i = i0; i < i1; ++i) {
+        const uint64_t w = kept_mass(i);
+        if (need < before + w) {
+            a.token[row] = base + i;
+            if (a.logprob) a.logprob[row] = (float)log((double)w / (double)total);
+            break;
         }
+        before += w;
     }
 }
 
 template <class T>
 static int launch(Args &a, cudaStream_t s) {
-    // static shared memory of the kernel beside the row's slice
-    constexpr size_t kRoom = 227 * 1024 - sizeof(Shared) - sizeof(Extra) - 1024;
-    const int sms = sm_count();
-    int C = cluster_size(a.B, sms, 8);
-    while (C < 8 && (size_t)(a.V + C - 1) / C * sizeof(T) > kRoom) C *= 2;
+    constexpr size_t kHead = (sizeof(Work) + 15) / 16 * 16, kRoom = 227 * 1024 - kHead;
+    int C = cluster_size(a.B, a.V, sm_count(), 8, 2048);
+    while (C < 8 && (size_t)(a.V + C - 1) / C * sizeof(T) > kRoom - 64) C *= 2;
     a.slice = ((a.V + C - 1) / C + 15) / 16 * 16;  // slices start 16-byte aligned when the row does
-    a.cached = (size_t)a.slice * sizeof(T) <= kRoom;
-    const size_t smem = a.cached ? (size_t)a.slice * sizeof(T) : 0;
-    if (launch_cluster(sample_kernel<T>, C, a.B, smem, s, a) != cudaSuccess) return ECC_ERR_LAUNCH;
+    const size_t bytes = (size_t)a.slice * sizeof(T);
+    const cudaError_t e = bytes <= kRoom ? launch_cluster(sample_kernel<T, true>, C, a.B, kHead + bytes, s, a)
+                                         : launch_cluster(sample_kernel<T, false>, C, a.B, kHead, s, a);
+    if (e != cudaSuccess) return ECC_ERR_LAUNCH;
     return launch_status();
 }
 
