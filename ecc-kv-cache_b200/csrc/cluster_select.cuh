@@ -266,8 +266,7 @@ static inline int cluster_size(int64_t rows, int64_t n, int sms, int most, int l
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_cluster(void (*kernel)(KArgs...), int c, int64_t rows, size_t smem, cudaStream_t s,
                                          Args &&...args) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && c > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(c * rows));

@@ -67,6 +67,7 @@ def _load():
             f"`make -C {os.path.join(os.path.dirname(_HERE), 'csrc')}` (sm_100a)")
     lib = ctypes.CDLL(library_path)
     p, i64, i32, f32, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+    pg = ctypes.POINTER(_Pages)  # takes a _Pages by reference
     sig = {
         "ecc_strerror": ([i32], ctypes.c_char_p),
         "ecc_version": ([], i32),
@@ -109,14 +110,14 @@ def _load():
         "ecc_lse_gather_merge": ([p, p, p, i64, i32, i32, p, i32, i32, ctypes.c_uint32, ctypes.c_longlong, p, i32,
                                   p], i32),
         "ecc_lse_exchange_merge_dev": ([p, p, p, i64, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
-        "ecc_compress_paged": ([p, i64, i64, i64, p, i64, i64, p, i64, i64, i64, p, i64, i64, i32, i32, i64, p, p, p,
+        "ecc_compress_paged": ([p, i64, i64, i64, p, i64, i64, p, i64, i64, i64, p, i64, i64, i32, i32, i64, pg, p, p,
                                 i32, p], i32),
-        "ecc_dequantize_paged": ([p, i64, i64, p, p, i64, i64, p, i32, i32, i64, p, p, i32, p], i32),
+        "ecc_dequantize_paged": ([p, i64, i64, p, p, i64, i64, p, i32, i32, i64, pg, p, i32, p], i32),
         "ecc_decode_paged_workspace_size": ([i32, i32, i32, i64, i32], sz),
-        "ecc_decode_paged": ([p, p, p, i64, i64, p, p, p, p, p, i64, i64, p, sz, i32, i32, i32, f32, i32, i32, i32, p],
+        "ecc_decode_paged": ([p, p, p, i64, i64, pg, p, p, p, p, i64, i64, p, sz, i32, i32, i32, f32, i32, i32, i32, p],
                              i32),
         "ecc_evict_paged_workspace_size": ([i64], sz),
-        "ecc_evict_paged": ([p, p, i64, i64, p, p, p, i64, i64, p, p, i64, i64, i64, p, i32, i32, i32, i32, i32, i32, p,
+        "ecc_evict_paged": ([p, p, i64, i64, pg, p, p, i64, i64, pg, p, i64, i64, i64, p, i32, i32, i32, i32, i32, i32, p,
                              sz, p], i32),
         "ecc_sample": ([p, i64, i32, i32, i64, p, p, f32, p, i32, p, f32, p, f32, p, p, p], i32),
         "ecc_lse_gather_merge_dev": ([p, p, p, i64, i32, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
@@ -879,30 +880,87 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 # ---------------------------------------------------------------------------
 # Paged cache: sequences of any lengths in pages of a shared pool
 # ---------------------------------------------------------------------------
-def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_table: torch.Tensor, B: int):
-    """Checks pools [pages, Hkv, page_size, R] and their page table [B, width]
-    int32; returns ((k strides), (v strides), ecc_pages_t)."""
-    ks = _pool_strides(k_pool, "k_pool")
-    if k_pool.dim() != 4:
-        raise RuntimeError("a paged pool must be [pages, Hkv, page_size, 128] (or [.., 96])")
-    vs = ks
-    if v_pool is not None:
-        vs = _pool_strides(v_pool, "v_pool")
-        if v_pool.shape != k_pool.shape or v_pool.device != k_pool.device:
-            raise RuntimeError("k_pool and v_pool must have the same shape and device")
-    _dev_int(block_table, "block_table", k_pool.device)
-    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1:
-        raise RuntimeError("block_table must be int32 [B, width] with contiguous rows, one row per sequence")
-    P, ps, width = k_pool.shape[0], k_pool.shape[2], block_table.shape[1]
-    if ps % 16 and width > 1:
-        raise RuntimeError(f"page_size must be a multiple of 16 (or one page per sequence), got {ps}")
-    return ks, vs, _Pages(block_table.data_ptr(), block_table.stride(0), width, ps, P)
+def _launch(fn, what: str, dev: torch.device, *args) -> None:
+    """fn(*args, current stream of dev) with dev the current device."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _check(rc, what)
 
 
-def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> None:
-    _dev_int(t, name, device)
-    if t.dim() != 1 or t.numel() != B or not t.is_contiguous():
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of B elements")
+def _scratch(workspace: torch.Tensor | None, dev: torch.device, need: int) -> torch.Tensor:
+    """The caller's workspace, checked, or one of the library's own: kept per
+    stream between eager calls, but fresh in a capture, whose memory then
+    belongs to that graph alone (graphs may run beside one another)."""
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous() \
+                or workspace.numel() * workspace.element_size() < need:
+            raise RuntimeError(f"workspace must be contiguous, on the pools' device and hold {need} bytes")
+        return workspace
+    with_dev = torch.cuda.current_device() == dev.index
+    if with_dev and not torch.cuda.is_current_stream_capturing():
+        ws = _ws_cache.get((dev.index, torch._C._cuda_getCurrentRawStream(dev.index)))
+        if ws is not None and ws.numel() >= need:
+            return ws
+        return _workspace(dev, need)
+    with torch.cuda.device(dev):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(need, dtype=torch.uint8, device=dev)
+        return _workspace(dev, need)
+
+
+def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None):
+    """Checks pools [pages, Hkv, page_size, R]; returns (shape, k strides and
+    v strides of a page and a head in records)."""
+    _require_cuda(k_pool, "k_pool")
+    shape = k_pool.shape
+    if k_pool.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in (BLOCK_BYTES, RECORD96):
+        raise RuntimeError("k_pool must be a uint8 pool [pages, Hkv, page_size, 128] (or [.., 96])")
+    strides = []
+    for t, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+        if t is None:
+            strides.append((0, 0))
+            continue
+        if t is not k_pool:
+            _require_cuda(t, name)
+            if t.shape != shape or t.dtype is not torch.uint8 or t.device != k_pool.device:
+                raise RuntimeError("k_pool and v_pool must have the same shape, type and device")
+        sp, sh, st, s1 = t.stride()
+        rb = shape[3]
+        if s1 != 1 or st != rb or sp % rb or sh % rb:
+            raise RuntimeError(f"{name}: a page's blocks must be contiguous {rb}-byte rows, page and head strides whole "
+                               f"blocks")
+        strides.append((sp // rb, sh // rb))
+    return shape, strides[0], strides[1]
+
+
+def _pages(table: torch.Tensor, name: str, B: int, shape, dev: torch.device) -> _Pages:
+    if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.device != dev:
+        raise RuntimeError(f"{name} must be an int32 tensor on the pools' device")
+    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or table.stride(1) != 1:
+        raise RuntimeError(f"{name} must be int32 [B, width] with contiguous rows, one row per sequence")
+    width = table.shape[1]
+    if shape[2] % 16 and width > 1:
+        raise RuntimeError(f"page_size must be a multiple of 16 (or one page per sequence), got {shape[2]}")
+    return _Pages(table.data_ptr(), table.stride(0), width, shape[2], shape[0])
+
+
+def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != device or t.dim() != 1 \
+            or t.shape[0] != B or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of B elements on the pools' device")
+    return t.data_ptr()
+
+
+def _weights_like(t: torch.Tensor, name: str, B: int, hkv: int, capacity: int, dev) -> tuple:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.dim() != 3 or t.device != dev \
+            or t.shape[0] != B or t.shape[1] != hkv or t.shape[2] < capacity or t.stride(2) != 1:
+        raise RuntimeError(f"{name} must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on the "
+                           f"pools' device")
+    return t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
@@ -917,31 +975,32 @@ def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.T
     None: ``k`` alone.  A position or page out of range writes nothing and
     raises the flag device_status() reports; two tokens of one call must not
     name the same slot."""
-    if k.dim() != 4:
-        raise RuntimeError("k must be float16 [B, Hkv, L, 128]")
     if (v is None) != (v_pool is None):
         raise RuntimeError("v and v_pool go together")
-    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, k.shape[0])
+    shape, ks, vs = _paged_pools(k_pool, v_pool)
+    dev = k_pool.device
+    strides = []
     for t, name in ((k, "k"), (v, "v")):
         if t is None:
+            strides.append((0, 0, 0, 1))
             continue
         _require_cuda(t, name)
-        if t.dtype != torch.float16 or t.shape[-1] != D or t.stride(-1) != 1 or t.shape != k.shape:
-            raise RuntimeError(f"{name} must be float16 [B, Hkv, L, 128] with a contiguous last dimension, k and v alike")
-        if t.shape[1] != k_pool.shape[1] or t.device != k_pool.device:
-            raise RuntimeError(f"{name} must have the pools' kv heads and device")
-    B, H, L, _ = k.shape
-    _per_sequence(pos, "pos", k.device, B)
-    if new_lens is not None:
-        _per_sequence(new_lens, "new_lens", k.device, B)
-    vargs = (None, 0, 0, 0, None, 0, 0) if v is None else (_ptr(v), v.stride(0), v.stride(1), v.stride(2),
-                                                           _ptr(v_pool), vs[0], vs[1])
-    with torch.cuda.device(k.device):
-        rc = _lib.ecc_compress_paged(_ptr(k), k.stride(0), k.stride(1), k.stride(2), _ptr(k_pool), ks[0], ks[1], *vargs,
-                                     B, H, L, ctypes.byref(pages), _ptr(pos),
-                                     None if new_lens is None else _ptr(new_lens), _cmode(rotate, k_pool, v_pool),
-                                     _stream(k))
-    _check(rc, "compress_pair_paged")
+        if t.dtype is not torch.float16 or t.dim() != 4 or t.shape != k.shape or t.device != dev:
+            raise RuntimeError(f"{name} must be float16 [B, Hkv, L, 128] on the pools' device, k and v alike")
+        st = t.stride()
+        if st[3] != 1:
+            raise RuntimeError(f"{name} must have a contiguous last dimension")
+        strides.append(st)
+    B, H, L, d = k.shape
+    if d != D or H != shape[1]:
+        raise RuntimeError("k and v must have the pools' kv heads and 128 dimensions")
+    pages = _pages(block_table, "block_table", B, shape, dev)
+    pos_p = _per_sequence(pos, "pos", dev, B)
+    new_p = None if new_lens is None else _per_sequence(new_lens, "new_lens", dev, B)
+    (kb, kh, kl, _), (vb, vh, vl, _) = strides
+    _launch(_lib.ecc_compress_paged, "compress_pair_paged", dev, k.data_ptr(), kb, kh, kl, k_pool.data_ptr(), ks[0], ks[1],
+            None if v is None else v.data_ptr(), vb, vh, vl, None if v is None else v_pool.data_ptr(), vs[0], vs[1],
+            B, H, L, pages, pos_p, new_p, (1 if rotate else 0) | (COMPRESS_BLOCK96 if shape[3] == RECORD96 else 0))
 
 
 def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_table: torch.Tensor,
@@ -951,26 +1010,22 @@ def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_ta
     behind them, with the inverse rotation applied (``unrotate``; one rounding
     at the end).  ``v_pool`` None gives k alone.  ``out``: tensors to write to,
     contiguous and of that shape."""
-    B = block_table.shape[0]
-    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
-    _per_sequence(seq_lens, "seq_lens", k_pool.device, B)
-    H, dev, n = k_pool.shape[1], k_pool.device, 1 if v_pool is None else 2
-    shape = (B, H, int(max_len), D)
+    shape, ks, vs = _paged_pools(k_pool, v_pool)
+    dev, B, H, n = k_pool.device, block_table.shape[0], shape[1], 1 if v_pool is None else 2
+    pages = _pages(block_table, "block_table", B, shape, dev)
+    lens = _per_sequence(seq_lens, "seq_lens", dev, B)
+    want = (B, H, int(max_len), D)
     if max_len < 0:
         raise RuntimeError("max_len must not be negative")
     if out is None:
-        out = tuple(torch.empty(shape, dtype=torch.float16, device=dev) for _ in range(n))
-    elif len(out) != n or any(tuple(t.shape) != shape or t.dtype != torch.float16 or not t.is_contiguous()
+        out = tuple(torch.empty(want, dtype=torch.float16, device=dev) for _ in range(n))
+    elif len(out) != n or any(tuple(t.shape) != want or t.dtype is not torch.float16 or not t.is_contiguous()
                               or t.device != dev for t in out):
         raise RuntimeError("out must hold contiguous float16 tensors [B, Hkv, max_len, 128] on the pools' device")
-    mode = (1 if unrotate else 0) | (2 if k_pool.shape[-1] == RECORD96 else 0)
-    with torch.cuda.device(dev):
-        rc = _lib.ecc_dequantize_paged(_ptr(k_pool), ks[0], ks[1], _ptr(out[0]),
-                                       None if v_pool is None else _ptr(v_pool), vs[0], vs[1],
-                                       None if v_pool is None else _ptr(out[1]), B, H, int(max_len),
-                                       ctypes.byref(pages), _ptr(seq_lens), mode, _stream(k_pool))
-    _check(rc, "dequantize_paged")
-    return out if v_pool is not None else out[0]
+    _launch(_lib.ecc_dequantize_paged, "dequantize_paged", dev, k_pool.data_ptr(), ks[0], ks[1], out[0].data_ptr(),
+            None if n == 1 else v_pool.data_ptr(), vs[0], vs[1], None if n == 1 else out[1].data_ptr(), B, H,
+            int(max_len), pages, lens, (1 if unrotate else 0) | (2 if shape[3] == RECORD96 else 0))
+    return out if n == 2 else out[0]
 
 
 def decode_paged_workspace_size(B: int, hq: int, hkv: int, capacity: int, with_weights: bool = False) -> int:
@@ -997,43 +1052,31 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     zero row (lse -inf) and adds no weight.  GQA groups of up to 8."""
     q3 = _query(query)
     B, hq, _ = q3.shape
-    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
+    shape, ks, vs = _paged_pools(k_pool, v_pool)
     if ks != vs:
         raise RuntimeError("k_pool and v_pool must have the same strides")
-    dev, hkv = k_pool.device, k_pool.shape[1]
+    dev, hkv = k_pool.device, shape[1]
     if q3.device != dev:
         raise RuntimeError("query and pools must be on the same device")
     if hq % hkv or hq // hkv > 8:
         raise RuntimeError(f"query heads ({hq}) must be 1 to 8 times the kv heads ({hkv})")
-    _per_sequence(seq_lens, "seq_lens", dev, B)
+    pages = _pages(block_table, "block_table", B, shape, dev)
+    lens = _per_sequence(seq_lens, "seq_lens", dev, B)
     if window < 0 or sinks < 0 or (sinks and not window):
         raise RuntimeError("window and sinks must not be negative, and sinks need a window")
     capacity = pages.width * pages.page_size
-    wargs = (None, 0, 0)
-    if weights is not None:
-        _require_cuda(weights, "weights")
-        if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, hkv) \
-                or weights.shape[2] < capacity or weights.stride(2) != 1 or weights.device != dev:
-            raise RuntimeError(f"weights must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on "
-                               f"the pools' device")
-        wargs = (_ptr(weights), weights.stride(0), weights.stride(1))
+    wp, wb, wh = (None, 0, 0) if weights is None else _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out is None:
         out = torch.empty((B, hq, 1, D), dtype=torch.float16, device=dev)
-    elif not out.is_contiguous() or out.dtype != torch.float16 or out.numel() != B * hq * D or out.device != dev:
+    elif not out.is_contiguous() or out.dtype is not torch.float16 or out.numel() != B * hq * D or out.device != dev:
         raise RuntimeError("out must be a contiguous float16 tensor of B*Hq*128 elements on the pools' device")
     lse = torch.empty((B, hq), dtype=torch.float32, device=dev) if return_lse else None
-    flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | _rec_flag(k_pool)
-    need = int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(weights is not None)))
-    with torch.cuda.device(dev):
-        ws = workspace if workspace is not None else _workspace(dev, need)
-        if ws.numel() * ws.element_size() < need or ws.device != dev:
-            raise RuntimeError(f"workspace too small or on another device: {need} bytes needed")
-        rc = _lib.ecc_decode_paged(_ptr(q3), _ptr(k_pool), _ptr(v_pool), ks[0], ks[1], ctypes.byref(pages),
-                                   _ptr(seq_lens), _ptr(out), None if lse is None else _ptr(lse), *wargs, _ptr(ws),
-                                   ws.numel() * ws.element_size(), B, hq, hkv,
-                                   float(sm_scale) if sm_scale is not None else 0.0, int(window), int(sinks), flags,
-                                   _stream(q3))
-    _check(rc, "decode_attention_paged")
+    flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | (BLOCK96 if shape[3] == RECORD96 else 0)
+    ws = _scratch(workspace, dev, _lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, weights is not None))
+    _launch(_lib.ecc_decode_paged, "decode_attention_paged", dev, q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+            ks[0], ks[1], pages, lens, out.data_ptr(), None if lse is None else lse.data_ptr(), wp, wb, wh, ws.data_ptr(),
+            ws.numel() * ws.element_size(), B, hq, hkv, 0.0 if sm_scale is None else float(sm_scale), int(window),
+            int(sinks), flags)
     return (out, lse) if return_lse else out
 
 
@@ -1056,45 +1099,35 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     were kept (-1 behind them).  The new lengths are seq_lens.clamp(max=budget);
     seq_lens itself is not changed, so that every layer can be cut by the same
     lengths."""
-    B = block_table.shape[0]
-    ks, vs, pages = _paged_pools(k_pool, v_pool, block_table, B)
-    ks2, _, outs = _paged_pools(k_pool, v_pool, out_table, B)
+    shape, ks, vs = _paged_pools(k_pool, v_pool)
     if ks != vs:
         raise RuntimeError("k_pool and v_pool must have the same strides")
-    dev, hkv, capacity = k_pool.device, k_pool.shape[1], pages.width * pages.page_size
-    _per_sequence(seq_lens, "seq_lens", dev, B)
+    dev, hkv, B = k_pool.device, shape[1], block_table.shape[0]
+    pages = _pages(block_table, "block_table", B, shape, dev)
+    outs = _pages(out_table, "out_table", B, shape, dev)
+    lens = _per_sequence(seq_lens, "seq_lens", dev, B)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise RuntimeError("budget must be positive and hold the sinks and the recent tokens")
     if outs.width * outs.page_size < budget:
         raise RuntimeError(f"out_table names fewer than {budget} tokens per sequence")
-    if out_table.data_ptr() == block_table.data_ptr():
+    if outs.table == pages.table:
         raise RuntimeError("out_table must name other pages than block_table")
+    capacity = pages.width * pages.page_size
+    wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out_weights is None:
-        out_weights = torch.empty((B, hkv, weights.shape[-1]), dtype=torch.float32, device=dev)
-    for t, name in ((weights, "weights"), (out_weights, "out_weights")):
-        _require_cuda(t, name)
-        if t.dtype != torch.float32 or t.dim() != 3 or tuple(t.shape[:2]) != (B, hkv) or t.shape[2] < capacity \
-                or t.stride(2) != 1 or t.device != dev:
-            raise RuntimeError(f"{name} must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on the "
-                               f"pools' device")
+        out_weights = torch.empty((B, hkv, weights.shape[2]), dtype=torch.float32, device=dev)
+    op, ob, oh = _weights_like(out_weights, "out_weights", B, hkv, capacity, dev)
     if out_weights.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
         raise RuntimeError("out_weights must not share memory with weights")
     if kept is None:
         kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
-    elif tuple(kept.shape) != (B, hkv, budget) or kept.dtype != torch.int32 or not kept.is_contiguous() \
+    elif tuple(kept.shape) != (B, hkv, budget) or kept.dtype is not torch.int32 or not kept.is_contiguous() \
             or kept.device != dev:
         raise RuntimeError("kept must be a contiguous int32 tensor [B, Hkv, budget] on the pools' device")
-    need = int(_lib.ecc_evict_paged_workspace_size(k_pool.shape[0]))
-    with torch.cuda.device(dev):
-        ws = workspace if workspace is not None else _workspace(dev, need)
-        if ws.numel() * ws.element_size() < need or ws.device != dev:
-            raise RuntimeError(f"workspace too small or on another device: {need} bytes needed")
-        rc = _lib.ecc_evict_paged(_ptr(k_pool), _ptr(v_pool), ks[0], ks[1], ctypes.byref(pages), _ptr(seq_lens),
-                                  _ptr(weights), weights.stride(0), weights.stride(1), ctypes.byref(outs),
-                                  _ptr(out_weights), out_weights.stride(0), out_weights.stride(1),
-                                  out_weights.shape[2], _ptr(kept), B, hkv, int(budget), int(sinks), int(recent),
-                                  k_pool.shape[-1], _ptr(ws), ws.numel() * ws.element_size(), _stream(k_pool))
-    _check(rc, "evict_paged")
+    ws = _scratch(workspace, dev, _lib.ecc_evict_paged_workspace_size(shape[0]))
+    _launch(_lib.ecc_evict_paged, "evict_paged", dev, k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1], pages, lens,
+            wp, wb, wh, outs, op, ob, oh, out_weights.shape[2], kept.data_ptr(), B, hkv, int(budget), int(sinks),
+            int(recent), shape[3], ws.data_ptr(), ws.numel() * ws.element_size())
     return out_weights, kept
 
 
@@ -1153,9 +1186,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     elif tuple(out.shape) != (B,) or out.dtype != torch.int64 or not out.is_contiguous() or out.device != dev:
         raise RuntimeError("out must be a contiguous int64 tensor [B] on the logits' device")
     logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprobs else None
-    with torch.cuda.device(dev):
-        rc = _lib.ecc_sample(_ptr(logits), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V, _ptr(uniform), t[0],
-                             float(t[1]), k[0], int(k[1]), p[0], float(p[1]), m[0], float(m[1]), _ptr(out),
-                             None if logprob is None else _ptr(logprob), _stream(logits))
-    _check(rc, "sample_tokens")
+    _launch(_lib.ecc_sample, "sample_tokens", dev, logits.data_ptr(), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V,
+            uniform.data_ptr(), t[0], float(t[1]), k[0], int(k[1]), p[0], float(p[1]), m[0], float(m[1]), out.data_ptr(),
+            None if logprob is None else logprob.data_ptr())
     return (out, logprob) if return_logprobs else out
