@@ -129,7 +129,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     const uint32_t bars = sbase + kSmBar + warp * kStages * 8;
 
     if (threadIdx.x < 16) {
-        const float cv = lm(threadIdx.x);
+        const float cv = lm(threadIdx.x) * kCentScale;
         const __half hi = __float2half_rn(cv);
         const __half lo = __float2half_rn(cv - __half2float(hi));
         s_cent[threadIdx.x] = (uint32_t)__half_as_ushort(hi) | ((uint32_t)__half_as_ushort(lo) << 16);
@@ -139,11 +139,8 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    for (int v = warp; v < 256; v += kWarps) {
-        const uint32_t e0 = s_cent[v & 15], e1 = s_cent[v >> 4];
-        reinterpret_cast<uint32_t *>(sm + kSmLut + v * 256)[lane] = __byte_perm(e0, e1, 0x5410);
-        reinterpret_cast<uint32_t *>(sm + kSmLut + v * 256 + 128)[lane] = __byte_perm(e0, e1, 0x7632);
-    }
+    for (int v = warp; v < 256; v += kWarps)
+        reinterpret_cast<uint2 *>(sm + kSmLut + v * 256)[lane] = lut_entry(s_cent, v, lane);
     pdl_trigger();
     pdl_wait();  // everything above touched shared memory only
 
@@ -204,14 +201,19 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         }
     };
 
-    // Pages of the next tile to fetch, looked up one tile ahead: lane 0 the
-    // whole tile's (or its first 16 tokens'), lane 1 the second 16 tokens'.
-    int p_tok = 0, p_page = 0;
-    auto look_up = [&]() {
-        const int tb = prod.st.base(prod.u) + 16 * (lane & 1);
-        const uint32_t pi = a.t.page_of(tb);
-        p_tok = tb - (int)pi * a.t.page_size;
-        if (lane < 2) p_page = pi < (uint32_t)a.t.width ? __ldg(a.t.table + (int64_t)prod.b * a.t.stride + pi) : 0;
+    // The next tile to fetch: slot p_slot of page p_page (lane 1, with two boxes a stage: of its second 16
+    // tokens), p_left tiles before the run of neighbouring tiles ends; the page after it is looked up early.
+    int p_slot, p_page, p_next = 0, p_pi, p_left;
+    const int *p_row;  // the sequence's row of the table
+    auto page_at = [&](int pi) { return pi < a.t.width ? __ldg(p_row + pi) : -1; };
+    auto start_run = [&]() {
+        const int tb = prod.st.base(prod.u) + (a.halves ? 16 * (lane & 1) : 0);
+        p_left = (prod.u < prod.st.nsink ? prod.st.nsink : prod.st.n) - prod.u;
+        p_row = a.t.table + (int64_t)prod.b * a.t.stride;
+        p_pi = (int)a.t.page_of(tb);
+        p_slot = tb - p_pi * a.t.page_size;
+        p_page = page_at(p_pi);
+        if (!a.halves) p_next = page_at(p_pi + 1);
     };
     auto issue_next = [&](int s, bool more) {
         const uint32_t bar = bars + 8 * s;
@@ -219,7 +221,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             fence_proxy_async();  // this warp's earlier reads of the stage precede the overwrite
             mbar_expect_tx(bar, kStageBytes);
         }
-        __syncwarp();
+        if (a.halves) __syncwarp();
         if (lane == 0 || (lane == 1 && a.halves)) {
             int page = p_page;
             if ((uint32_t)page >= (uint32_t)a.t.n_pages) {
@@ -230,20 +232,39 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             }
             const uint32_t dst = ring + s * kStageBytes;
             if (a.halves) fence_proxy_async();
-            tma_4d(dst + kOffKC + lane * kSubC, &mkc, 0, p_tok, prod.h, page, bar);
-            tma_4d(dst + kOffKS + lane * kSubS, &mks, 64, p_tok, prod.h, page, bar);
-            tma_4d(dst + kOffVC + lane * kSubC, &mvc, 0, p_tok, prod.h, page, bar);
-            tma_4d(dst + kOffVS + lane * kSubS, &mvs, 64, p_tok, prod.h, page, bar);
+            tma_4d(dst + kOffKC + lane * kSubC, &mkc, 0, p_slot, prod.h, page, bar);
+            tma_4d(dst + kOffKS + lane * kSubS, &mks, 64, p_slot, prod.h, page, bar);
+            tma_4d(dst + kOffVC + lane * kSubC, &mvc, 0, p_slot, prod.h, page, bar);
+            tma_4d(dst + kOffVS + lane * kSubS, &mvs, 64, p_slot, prod.h, page, bar);
         }
-        if (more) {
-            if (++prod.u == prod.st.n) advance_row(prod);
-            look_up();
+        if (!more) return;
+        ++prod.u;
+        if (--p_left == 0) {
+            if (prod.u == prod.st.n) advance_row(prod);
+            start_run();
+        } else if (a.halves) {
+            p_slot += kTile;
+            if (p_slot >= a.t.page_size) {  // by one or two pages
+                do {
+                    p_slot -= a.t.page_size;
+                    ++p_pi;
+                } while (p_slot >= a.t.page_size);
+                p_page = page_at(p_pi);
+            }
+        } else {
+            p_slot += kTile;
+            if (p_slot == a.t.page_size) {
+                p_slot = 0;
+                p_page = p_next;
+                p_next = page_at(++p_pi + 1);
+            }
         }
     };
 
-    Lane<G> L;
+    Lane<G, true> L;
     L.g = lane >> 2;
     L.c = lane & 3;
+    L.scale_log2_0 = a.scale_log2;
     // query words of lane (g, c): dims 32c.. of query head g of the group (as in decode_tma_kernel)
     auto load_q = [&](uint4 (&qw)[4], int b, int h) {
         const int qh = (G <= 4) ? (L.g & 3) : L.g;
@@ -254,15 +275,15 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     {
         uint4 qw[4];
         load_q(qw, cons.b, cons.h);
-        look_up();
+        start_run();
         for (int s = 0; s < kStages && s < ntiles; ++s) issue_next(s, s + 1 < ntiles);
         L.set_query(qw, (a.flags & ECC_DECODE_ROTATE_Q) != 0);
     }
-    L.lane4 = (uint32_t)lane * 4u;
+    L.lane8 = (uint32_t)lane * 8u;
+    L.lane_hi = lane_hi_of(lane);
     L.sel_half = (L.g & 1) ? 0x7632u : 0x5410u;
     L.voff = 16u * (uint32_t)((L.g >> 1) ^ L.c) + 8u * (uint32_t)(L.g & 1);
     L.soff = 16u * (uint32_t)((L.g >> 2) & 1);
-    L.scale_log2 = a.scale_log2;
     bool ok = true;
     int jfail = -1, j = 0, stage = 0;
     uint32_t phase = 0;
@@ -271,6 +292,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         const int seg_tiles = min(ntiles - j, cons.st.n - cons.u);
         const int row = cons.b * Hkv + cons.h;
         const bool begins = cons.u == 0, ends = cons.u + seg_tiles == cons.st.n;
+        int tb = cons.st.base(cons.u);  // first token of the tile
         if (j > 0) {
             uint4 qw[4];
             load_q(qw, cons.b, cons.h);
@@ -298,9 +320,9 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             if (ok && !ready) jfail = j;
             ok = ok && ready;
             if (ok) {
-                const int tb = cons.st.base(cons.u);
-                const SeeBits see{cons.st.visible(tb, a.sinks)};
-                if (see.m != 0xffffffffu) {
+                SeeBits see{0xffffffffu};
+                if (tb + kTile > cons.st.len || tb < cons.st.ws) {
+                    see.m = cons.st.visible(tb, a.sinks);
                     // Slots behind the last token hold whatever was there before: their V metadata (it may
                     // read as NaN or infinity) is cleared, so that 0 probability times it stays 0.  Lane =
                     // token; chunk 1 of its row in the swizzled box (see Lane::load_v).
@@ -318,7 +340,8 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             __syncwarp();
             if (ok && j + kStages < ntiles) issue_next(stage, j + kStages + 1 < ntiles);
             ++j;
-            ++cons.u;
+            tb += kTile;
+            if (++cons.u == cons.st.nsink) tb = kTile * cons.st.w0;
             if (++stage == kStages) {
                 stage = 0;
                 phase ^= 1u;

@@ -197,15 +197,58 @@ struct NoScores {
     __device__ __forceinline__ void operator()(const float (&)[4], const float (&)[4]) const {}
 };
 
-// Consumer lane state for one work item.  For groups of at most 4 query heads
+// ---- the paired table (Lane<G, true>) ---------------------------------------
+// The centroids times kCentScale: of all factors, the one with which the eight
+// magnitudes lie nearest to fp16 values (8.6e-5 relative at most, 6.0e-5 rms
+// over normal data, where an fp16 rounding is 2^-11 at most and 2.2e-4 rms), so
+// that the fp16 parts alone serve the values: the output is rounded to fp16
+// once more anyway.  Keys take both parts.
+//
+// Row v (256 bytes) holds a pair of words per lane at v*256 + 8*lane, the hi
+// words and the lo words of the two codes of byte v; lanes 16..31 have them the
+// other way round.  One 64-bit load brings a key byte's pair into the registers
+// of operand rows g and g + 8, whose products are added up, so their order does
+// not matter; the 32-bit loads of the values' hi words (at lane_hi) then hit 32
+// distinct banks as well.
+constexpr float kCentScale = 0x1.61a50cp+0f;
+__device__ __forceinline__ uint2 lut_pair(uint32_t word, int byte_idx, uint32_t lane8) {
+    uint2 r;
+    const uint32_t a = __byte_perm(word, lane8, 0x5504u | ((uint32_t)byte_idx << 4));
+    asm("ld.shared.v2.u32 {%0, %1}, [%2+%3];" : "=r"(r.x), "=r"(r.y) : "r"(a), "n"(kSmemReserve + kSmLut));
+    return r;
+}
+__device__ __forceinline__ uint32_t lut_hi(uint32_t word, int byte_idx, uint32_t lane_hi) {
+    uint32_t r;
+    const uint32_t a = __byte_perm(word, lane_hi, 0x5504u | ((uint32_t)byte_idx << 4));
+    asm("ld.shared.u32 %0, [%1+%2];" : "=r"(r) : "r"(a), "n"(kSmemReserve + kSmLut));
+    return r;
+}
+__device__ __forceinline__ uint32_t lane_hi_of(int lane) { return 8u * lane + (lane < 16 ? 0u : 4u); }
+// This lane's pair of row v from the 16 packed centroids (hi | lo << 16).
+__device__ __forceinline__ uint2 lut_entry(const uint32_t *cent, int v, int lane) {
+    const uint32_t e0 = cent[v & 15], e1 = cent[v >> 4];
+    const uint32_t hi = __byte_perm(e0, e1, 0x5410), lo = __byte_perm(e0, e1, 0x7632);
+    return lane < 16 ? make_uint2(hi, lo) : make_uint2(lo, hi);
+}
+
+// Two e5m2 values (the top bytes of fp16 values) of bytes 2j, 2j + 1 of w as an fp16x2 word.
+__device__ __forceinline__ uint32_t e5m2_pair(uint32_t w, int j) { return __byte_perm(w, 0u, j ? 0x3424u : 0x1404u); }
+
+// Consumer lane state for one work item.  kFine: the paired table above, and
+// a query that is scaled to a largest magnitude in [1, 2) and, when it is
+// rotated here, not rounded to fp16 but carried as fp16 plus remainder (for
+// groups of up to 4 heads in the idle columns 4..7 of the QK operand,
+// otherwise as e5m2 words).  For groups of at most 4 query heads
 // the PV products use the idle columns 4..7 of the n8 operand for the V sign
 // term: lanes g < 4 of the P operand carry p * vscale of head g (columns
 // 0..3, centroid products), lanes g >= 4 carry 2 p * valpha of head g - 4
 // (columns 4..7, sign-bit products with the bits masked in place, so each
 // accumulator row has one power-of-two weight, removed at the end).
-template <int G>
+template <int G, bool kFine = false>
 struct Lane {
+    static constexpr bool kLoCols = kFine && G <= 4, kLoWords = kFine && G > 4;
     uint32_t qc[8][2];
+    uint32_t ql[kLoWords ? 8 : 1];  // remainders of the four values of qc[m], e5m2
     uint32_t qs[8][2];  // q of the sign products, k slot of bit p scaled by 2^-(ssh + kexp(p))
     float sgn2;         // 2^(ssh + 1): q.s = sgn2 * (sign product) - sum(q)
     float qsum[2];
@@ -217,7 +260,9 @@ struct Lane {
     uint32_t voff;  // this lane's byte offset in the swizzled V code box (see load_v)
     uint32_t soff;  // this lane's byte offset in the swizzled syndrome boxes (see qk, load_v)
     int g, c;
-    float scale_log2;
+    float scale_log2;   // of the scores, with the query's scaling
+    float scale_log2_0;  // kFine: without it
+    uint32_t lane8, lane_hi;  // kFine: offsets in the paired table
 
     // Query fragments of a row segment from the lane's fp16 query words qw
     // (dims 32c..32c+31 of its head): the centroid operand qc, the sign
@@ -257,7 +302,27 @@ struct Lane {
                 const float v = x[k];
                 const float q0 = __fmul_rn(v, kInvSqrt128);
                 const float rem = __fmaf_rn(-q0, kSqrt128, v);
-                x[k] = __half2float(__float2half_rn(__fmaf_rn(rem, kInvSqrt128, q0)));
+                x[k] = __fmaf_rn(rem, kInvSqrt128, q0);
+                if (!kFine) x[k] = __half2float(__float2half_rn(x[k]));
+            }
+        }
+        if constexpr (kFine) {
+            float qmax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) qmax = fmaxf(qmax, fabsf(x[k]));
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, off));
+            const int e2 = qmax > 0.0f ? max(-100, min(100, ((__float_as_int(qmax) >> 23) & 0xff) - 127)) : 0;
+            const float down = __int_as_float((127 - e2) << 23);
+            scale_log2 = scale_log2_0 * __int_as_float((127 + e2) << 23);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] *= down;
+        }
+        if constexpr (kLoCols) {  // lanes g >= 4 hold the remainders of head g - 4
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                const float hi = __half2float(__float2half_rn(x[k]));
+                x[k] = g < 4 ? hi : x[k] - hi;
             }
         }
 #pragma unroll
@@ -277,6 +342,22 @@ struct Lane {
             const int e2 = (qmax > 0.0f) ? ((__float_as_int(qmax) >> 23) & 0xff) - 127 : 0;
             const int ssh = max(0, e2);
             sgn2 = __int_as_float((ssh + 1 + 127) << 23);
+            if constexpr (kLoWords) {
+                // a remainder is at most 2^-11; an e5m2 keeps three bits of it down to 2^-14 and steps of 2^-16
+                // below, so at most 2^-14 of the fp16 rounding's 2^-11 is left
+#pragma unroll
+                for (int m = 0; m < 8; ++m) {
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float v = x[4 * m + j];
+                        // fp16, rounded to its top byte
+                        const uint32_t hw = __half_as_ushort(__float2half_rn(v - __half2float(__float2half_rn(v))));
+                        w |= ((hw + 0x7fu + ((hw >> 8) & 1u)) >> 8 & 0xffu) << (8 * j);
+                    }
+                    ql[m] = w;
+                }
+            }
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
                 const float f0 = __int_as_float((127 - ssh - kexp(2 * m)) << 23);
@@ -351,12 +432,18 @@ struct Lane {
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
             const int w = m >> 1, by = 2 * (m & 1);
-            const uint2 xa = lut(kwa[w], by, lane4);      // token g, k slots 2c, 2c+1
-            const uint2 ya = lut(kwa[w], by + 1, lane4);  // token g, k slots 2c+8, 2c+9
-            const uint2 xb = lut(kwb[w], by, lane4);      // token g+8
-            const uint2 yb = lut(kwb[w], by + 1, lane4);
+            // token g, k slots 2c, 2c+1 and 2c+8, 2c+9, then token g+8
+            const uint2 xa = kFine ? lut_pair(kwa[w], by, lane8) : lut(kwa[w], by, lane4);
+            const uint2 ya = kFine ? lut_pair(kwa[w], by + 1, lane8) : lut(kwa[w], by + 1, lane4);
+            const uint2 xb = kFine ? lut_pair(kwb[w], by, lane8) : lut(kwb[w], by, lane4);
+            const uint2 yb = kFine ? lut_pair(kwb[w], by + 1, lane8) : lut(kwb[w], by + 1, lane4);
             mma16816(sa, xa.x, xa.y, ya.x, ya.y, qc[m][0], qc[m][1]);
             mma16816(sb, xb.x, xb.y, yb.x, yb.y, qc[m][0], qc[m][1]);
+            if constexpr (kLoWords) {
+                const uint32_t l0 = e5m2_pair(ql[m], 0), l1 = e5m2_pair(ql[m], 1);
+                mma16816(sa, xa.x, xa.y, ya.x, ya.y, l0, l1);
+                mma16816(sb, xb.x, xb.y, yb.x, yb.y, l0, l1);
+            }
             mma16816(ss, kbits(ksa, ka5, ka10, ka1, 2 * m), kbits(ksb8, kb5, kb10, kb1, 2 * m),
                      kbits(ksa, ka5, ka10, ka1, 2 * m + 1), kbits(ksb8, kb5, kb10, kb1, 2 * m + 1), qs[m][0],
                      qs[m][1]);
@@ -364,13 +451,18 @@ struct Lane {
         // q.C of token g (head 2c+e) = hi row + lo row
         const float sc[4] = {sa[0] + sa[2], sa[1] + sa[3], sb[0] + sb[2], sb[1] + sb[3]};
         // score = scale q.C + alpha (2 q.b - sum q) + zero sum q  (s = 2b - 1)
-        const float k_sa = h_lo(kma.x), k_za = h_hi(kma.x), k_aa = h_lo(kma.y);
-        const float k_sb = h_lo(kmb.x), k_zb = h_hi(kmb.x), k_ab = h_lo(kmb.y);
+        constexpr float kUnit = kFine ? 1.0f / kCentScale : 1.0f;  // of the table's centroids
+        const float k_sa = h_lo(kma.x) * kUnit, k_za = h_hi(kma.x), k_aa = h_lo(kma.y);
+        const float k_sb = h_lo(kmb.x) * kUnit, k_zb = h_hi(kmb.x), k_ab = h_lo(kmb.y);
         const float k_ga = k_aa * sgn2, k_gb = k_ab * sgn2, k_da = k_za - k_aa, k_db = k_zb - k_ab;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float xa = fmaf(k_sa, sc[e], fmaf(k_ga, ss[e], k_da * qsum[e]));
-            const float xb = fmaf(k_sb, sc[2 + e], fmaf(k_gb, ss[2 + e], k_db * qsum[e]));
+            float xa = fmaf(k_sa, sc[e], fmaf(k_ga, ss[e], k_da * qsum[e]));
+            float xb = fmaf(k_sb, sc[2 + e], fmaf(k_gb, ss[2 + e], k_db * qsum[e]));
+            if constexpr (kLoCols) {  // linear in q: fp16 part plus remainder, in both lanes alike
+                xa += __shfl_xor_sync(0xffffffffu, xa, 2);
+                xb += __shfl_xor_sync(0xffffffffu, xb, 2);
+            }
             s2[e] = va ? xa * scale_log2 : -INFINITY;
             s2[2 + e] = vb8 ? xb * scale_log2 : -INFINITY;
         }
@@ -396,8 +488,9 @@ struct Lane {
     // g + 8 of accumulator i), four products: centroids hi x ws, centroids
     // lo x ws, centroids hi x residual, signs x sign weights.
     __device__ __forceinline__ void pv(const VRaw &v, const float (&p)[4]) {
-        const float v_sa = h_lo(v.vma.x), v_aa = h_lo(v.vma.y);
-        const float v_sb = h_lo(v.vmb.x), v_ab = h_lo(v.vmb.y);
+        constexpr float kUnit = kFine ? 1.0f / kCentScale : 1.0f;
+        const float v_sa = h_lo(v.vma.x) * kUnit, v_aa = h_lo(v.vma.y);
+        const float v_sb = h_lo(v.vmb.x) * kUnit, v_ab = h_lo(v.vmb.y);
         constexpr bool kSplitCols = G <= 4;
         // rows of the pre-transpose matrices: t = 0 token g, t = 1 token g+8
         uint32_t mw[2], mr[2], ma[2];
@@ -438,18 +531,27 @@ struct Lane {
             constexpr uint32_t kLo = 0x0F0F0F0Fu, kHi = 0xF0F0F0F0u;
             const uint32_t ia_e = (xa0 & kLo) | ((xa1 << 4) & kHi), ia_o = ((xa0 >> 4) & kLo) | (xa1 & kHi);
             const uint32_t ib_e = (xb0 & kLo) | ((xb1 << 4) & kHi), ib_o = ((xb0 >> 4) & kLo) | (xb1 & kHi);
-            uint2 r0[4], r1[4], r2[4], r3[4];
+            uint2 r0[4], r1[4], r2[4], r3[4];  // kFine: the hi words alone
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                r0[k] = lut(ia_e, k, lane4);
-                r1[k] = lut(ia_o, k, lane4);
-                r2[k] = lut(ib_e, k, lane4);
-                r3[k] = lut(ib_o, k, lane4);
+                if constexpr (kFine) {
+                    r0[k].x = lut_hi(ia_e, k, lane_hi);
+                    r1[k].x = lut_hi(ia_o, k, lane_hi);
+                    r2[k].x = lut_hi(ib_e, k, lane_hi);
+                    r3[k].x = lut_hi(ib_o, k, lane_hi);
+                } else {
+                    r0[k] = lut(ia_e, k, lane4);
+                    r1[k] = lut(ia_o, k, lane4);
+                    r2[k] = lut(ib_e, k, lane4);
+                    r3[k] = lut(ib_o, k, lane4);
+                }
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) mma16816(o[4 * w + k], r0[k].x, r1[k].x, r2[k].x, r3[k].x, bw[0], bw[1]);
+            if constexpr (!kFine) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma16816(o[4 * w + k], r0[k].y, r1[k].y, r2[k].y, r3[k].y, bw[0], bw[1]);
+                for (int k = 0; k < 4; ++k) mma16816(o[4 * w + k], r0[k].y, r1[k].y, r2[k].y, r3[k].y, bw[0], bw[1]);
+            }
 #pragma unroll
             for (int k = 0; k < 4; ++k) mma16816(o[4 * w + k], r0[k].x, r1[k].x, r2[k].x, r3[k].x, br[0], br[1]);
 #pragma unroll
