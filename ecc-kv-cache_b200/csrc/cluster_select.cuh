@@ -43,7 +43,8 @@ struct alignas(16) Shared {
     uint32_t cta_a, cta_b;  // totals of this CTA, read by the cluster
     uint64_t cta64;
     CrossingShared cross;
-    uint32_t cut;  // written by the CTA that finds it
+    uint32_t cut;     // written by the CTA that finds it
+    uint32_t listed;  // entries of the first CTA's list
 };
 
 // Ascending order of floats as ascending unsigned order; -0 equals +0.
@@ -259,6 +260,25 @@ static inline int cluster_size(int64_t rows, int64_t n, int sms, int most, int l
     int c = 1;
     while (c < most && rows * (2 * c) <= sms && n >= (int64_t)least * 2 * c) c *= 2;
     return c;
+}
+
+// Entries of a list of 64-bit words in the place of a pass's bins.
+constexpr int kList = sizeof(Shared::hist) / 8;
+
+// Descending sort of the first power of two >= n entries (those from n on must
+// be zero) of `x` by the whole block.
+__device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
+    int size = 1;
+    while (size < n) size *= 2;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+                const int i = 2 * t - (t & (j - 1));  // bit j of i is clear
+                const unsigned long long p = x[i], q = x[i + j];
+                if ((p < q) == ((i & k) == 0)) x[i] = q, x[i + j] = p;
+            }
+            __syncthreads();
+        }
 }
 
 // Launch with a cluster of `c` CTAs per row (y), as a dependent of the kernel

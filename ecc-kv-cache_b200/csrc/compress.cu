@@ -773,7 +773,9 @@ __global__ void __launch_bounds__(kCompressWarps * 32, 3) compress_kernel(const 
             if (next >= t0) load_vec(jobs.j[1], next - t0, nraw, nref, off1, en1, pages);
             else load_vec(jobs.j[0], next, nraw, nref, off0, en0, pages);
         }
-        if (!compress_fast<kRotate>(raw, ref, tabq, red, st)) {
+        // a warp without a vector to write (padding of a ragged batch) has nothing to compute
+        const bool idle = kPaged && !__any_sync(kFull, ref.valid);
+        if (!idle && !compress_fast<kRotate>(raw, ref, tabq, red, st)) {
             const bool second = tile >= t0;  // block-uniform
             const CompressJob &jb = second ? jobs.j[1] : jobs.j[0];
             const uint32_t t = second ? tile - t0 : tile;

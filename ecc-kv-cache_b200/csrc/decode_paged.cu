@@ -39,7 +39,6 @@ constexpr int kMaxBatch = ECC_PAGED_MAX_BATCH;
 constexpr int kSmPrefix = kSmBytes;                        // [kMaxBatch + 1] int
 constexpr int kSmPaged = kSmPrefix + 4 * (kMaxBatch + 4);  // total
 static_assert(kSmPaged <= 227 * 1024, "shared memory budget");
-constexpr int kMergeGroups = 4;
 constexpr int kMaxRanges = 4096;  // warps of a launch at most (merge weights in shared memory)
 
 struct DecodeArgs {
@@ -405,6 +404,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
 // groups of 128 threads (a thread per dimension) each take every
 // kMergeGroups-th partial, so a long row (up to one partial per warp of the
 // GPU) is read with enough loads in flight.  Every sum has a fixed order.
+template <int kMergeGroups>
 __global__ void __launch_bounds__(kD *kMergeGroups)
 paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ out, float *__restrict__ lse,
                    float *__restrict__ lse2) {
@@ -461,7 +461,9 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
     s_o[grp][d] = acc;
     __syncthreads();
     if (grp == 0) {
-        float v = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+        float v = s_o[0][d];
+#pragma unroll
+        for (int k = 1; k < kMergeGroups; ++k) v += s_o[k][d];
         v = Ls > 0.0f ? v / Ls : 0.0f;
         if (a.flags & ECC_DECODE_UNROTATE_OUT) {
 #pragma unroll
@@ -469,7 +471,7 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
                 const float p = __shfl_xor_sync(0xffffffffu, v, s);
                 v = (lane & s) ? p - v : v + p;
             }
-            s_o[0][d] = v;
+            s_o[0][d] = v;  // (each thread reads its own sum only above)
             asm volatile("bar.sync 1, 128;" ::: "memory");
             const float x0 = s_o[0][lane], x1 = s_o[0][lane + 32], x2 = s_o[0][lane + 64], x3 = s_o[0][lane + 96];
             const float y0 = (warp & 1) ? x0 - x1 : x0 + x1, y1 = (warp & 1) ? x2 - x3 : x2 + x3;
@@ -684,9 +686,15 @@ extern "C" int ecc_decode_paged(const void *q_f16, const void *k_blocks, const v
 #undef ECC_PAGED_CASE
     }
     if (rc != ECC_OK) return rc;
-    if (launch_pdl(paged_merge_kernel, dim3((unsigned)(B * Hq)), dim3(kD * kMergeGroups), 0, s, a,
-                   reinterpret_cast<__half *>(out_f16), lse, weights ? lse2 : nullptr) != cudaSuccess)
-        return ECC_ERR_LAUNCH;
+    // partials per row when the rows are alike; a CTA of one group joins a few of them as fast and three times as
+    // many such CTAs fit an SM (B32 Hq32, 8 partials a row: MERGE_A us against MERGE_B)
+    const bool wide = l.slots / ((int64_t)B * Hkv) > 8;
+    const cudaError_t e =
+        wide ? launch_pdl(paged_merge_kernel<4>, dim3((unsigned)(B * Hq)), dim3(kD * 4), 0, s, a,
+                          reinterpret_cast<__half *>(out_f16), lse, weights ? lse2 : nullptr)
+             : launch_pdl(paged_merge_kernel<1>, dim3((unsigned)(B * Hq)), dim3(kD), 0, s, a,
+                          reinterpret_cast<__half *>(out_f16), lse, weights ? lse2 : nullptr);
+    if (e != cudaSuccess) return ECC_ERR_LAUNCH;
     rc = launch_status();
     if (rc != ECC_OK || !weights) return rc;
     switch (G) {

@@ -115,10 +115,58 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
         __syncthreads();
     }
     auto key = [&](int i) { return cached ? cache[i] : weight_key(__ldg(w + base + i)); };
-    uint32_t ties, equal;
-    const uint32_t kth = sel::kth_largest(sh, cl, key, n, (uint32_t)k, 0, &ties, &equal);
-    uint32_t cut = 0xffffffffu;
-    if (ties < equal) cut = sel::tie_cut(sh, cl, n, base, ties, [&](int i) { return key(i) == kth; });
+    // What is kept: keys above kth, equal ones below the position cut.  One pass counts the keys by exponent and
+    // six bits of mantissa, from 2^-23 to 2^8 (what lies outside falls into the end bins: the order is kept);
+    // the bin that holds the k-th key is then listed and sorted in the cluster's first CTA.  A bin that does not
+    // fit the list (many equal weights) is descended digit by digit.
+    uint32_t kth, cut = 0xffffffffu;
+    constexpr uint32_t kLowest = 0x80000000u + ((127u - 23u) << 23);
+    auto bin_of = [](uint32_t x) {  // 0: the largest
+        return sel::kBins - 1 - (int)min((uint32_t)sel::kBins - 1, x > kLowest ? (x - kLowest) >> 17 : 0u);
+    };
+    for (int i = tid; i < sel::kBins; i += sel::kThreads) sh.hist[i] = 0;
+    if (tid == 0) sh.listed = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < n; i += sel::kThreads) atomicAdd(&sh.hist[bin_of(key(i))], 1u);
+    cl.sync();
+    sel::cluster_share(cl, sh.hist, sh.tot);
+    sel::share_sums(sh.cross, cl, sh.tot, sh.warp64);
+    const sel::Crossing at_k = sel::crossing(sh.cross, cl, sh.tot, (uint64_t)k, sh.warp64);
+    if (at_k.here <= sel::kList) {
+        unsigned long long *list = reinterpret_cast<unsigned long long *>(sh.hist);
+        for (int i0 = tid - lane; i0 < n; i0 += sel::kThreads) {
+            const uint32_t x = i0 + lane < n ? key(i0 + lane) : 0;
+            const bool hit = i0 + lane < n && bin_of(x) == (int)at_k.slot;
+            const uint32_t m = __ballot_sync(0xffffffffu, hit);
+            if (!m) continue;
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(sel::of_rank(cl, &sh.listed, 0), (uint32_t)__popc(m));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
+            if (hit) sel::of_rank(cl, list, 0)[at] = ((unsigned long long)x << 32) | (uint32_t)~(uint32_t)(base + i0 + lane);
+        }
+        cl.sync();
+        if (rank == 0) {
+            const int m = (int)sh.listed;
+            int size = 1;
+            while (size < m) size *= 2;
+            for (int i = m + tid; i < size; i += sel::kThreads) list[i] = 0;
+            __syncthreads();
+            sel::sort_descending(list, m);
+            if (tid < C) {
+                const unsigned long long e = list[k - (int)at_k.before - 1];
+                *sel::of_rank(cl, &sh.cta_b, tid) = (uint32_t)(e >> 32);
+                *sel::of_rank(cl, &sh.cut, tid) = ~(uint32_t)e + 1;
+            }
+        }
+        cl.sync();
+        kth = sh.cta_b;
+        cut = sh.cut;
+    } else {
+        uint32_t ties, equal;
+        kth = sel::kth_largest(sh, cl, key, n, (uint32_t)k, 0, &ties, &equal);
+        if (ties < equal) cut = sel::tie_cut(sh, cl, n, base, ties, [&](int i) { return key(i) == kth; });
+    }
     auto keep = [&](int i) {
         const uint32_t x = key(i);
         return x > kth || (x == kth && (uint32_t)(base + i) < cut);

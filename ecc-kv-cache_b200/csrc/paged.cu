@@ -59,49 +59,63 @@ __global__ void __launch_bounds__(kReadWarps * 32, 3) dequant_paged_kernel(const
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & 3;
     const float2 *mytab = tab + (lane & 15);
     const uint32_t tiles = (a.n_vec + kReadTile - 1) / kReadTile;
-    for (uint32_t it = blockIdx.x; it < tiles * a.njobs; it += gridDim.x) {
+    // A lane's share of a vector: its code words, the syndrome, the metadata; a step's are requested before the
+    // step in front of it is worked on.
+    struct Raw {
+        uint32_t cw[4];
+        uint4 sy;
+        uint2 meta;
+        bool live;  // else: behind the sequence's last token
+    };
+    auto request = [&](uint32_t it, Raw &r) {
         const ReadJob &jb = it < tiles ? a.j[0] : a.j[1];
         const uint32_t vi = (it < tiles ? it : it - tiles) * kReadTile + warp * 8 + (lane >> 2);
-        const bool valid = vi < a.n_vec;
-        const uint32_t v = valid ? vi : 0u;
-        const uint32_t row = fdiv(v, a.div_l);
-        const int t = (int)(v - row * a.div_l.d);
+        r.live = false;
+        if (vi >= a.n_vec) return;
+        const uint32_t row = fdiv(vi, a.div_l);
+        const int t = (int)(vi - row * a.div_l.d);
         const uint32_t b = fdiv(row, a.div_h);
         const int h = (int)(row - b * a.div_h.d);
-        const uint8_t *src = nullptr;
-        {
-            const int n = __ldg(a.lens + b);
-            if (n < 0 || n > a.t.capacity) atomicExch(&g_paged_error, 5);
-            int slot;
-            if (t < min(n, a.t.capacity)) {
-                const int page = a.t.page((int)b, t, slot);
-                if (page >= 0) src = jb.blocks + ((int64_t)page * jb.bs_p + (int64_t)h * jb.bs_h + slot) * a.rec;
-            }
-        }
+        const int n = __ldg(a.lens + b);
+        if (n < 0 || n > a.t.capacity) atomicExch(&g_paged_error, 5);
+        if (t >= min(n, a.t.capacity)) return;
+        int slot;
+        const int page = a.t.page((int)b, t, slot);
+        if (page < 0) return;
+        const uint8_t *src = jb.blocks + ((int64_t)page * jb.bs_p + (int64_t)h * jb.bs_h + slot) * a.rec;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) r.cw[c] = __ldg(reinterpret_cast<const uint32_t *>(src) + 4 * c + g);
+        r.sy = __ldg(reinterpret_cast<const uint4 *>(src + kSynOff));
+        r.meta = __ldg(reinterpret_cast<const uint2 *>(src + kScaleOff));
+        r.live = true;
+    };
+    const uint32_t steps = tiles * a.njobs;
+    Raw next;
+    if (blockIdx.x < steps) request(blockIdx.x, next);
+    for (uint32_t it = blockIdx.x; it < steps; it += gridDim.x) {
+        const Raw cur = next;
+        if (it + gridDim.x < steps) request(it + gridDim.x, next);
+        const uint32_t v = (it < tiles ? it : it - tiles) * kReadTile + warp * 8 + (lane >> 2);
+        const bool valid = v < a.n_vec;
+        __half *const out = it < tiles ? a.j[0].out : a.j[1].out;
         float2 P[4][4];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int j = 0; j < 4; ++j) P[c][j] = make_float2(0.0f, 0.0f);
-        if (src) {
-            uint32_t cw[4], sy[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                cw[c] = __ldg(reinterpret_cast<const uint32_t *>(src) + 4 * c + g);
-                sy[c] = __ldg(reinterpret_cast<const uint32_t *>(src + kSynOff) + c);
-            }
-            const uint2 m = __ldg(reinterpret_cast<const uint2 *>(src + kScaleOff));
-            const float sc = __half2float(__ushort_as_half((unsigned short)(m.x & 0xffffu))) * a.norm;
-            const float zr = __half2float(__ushort_as_half((unsigned short)(m.x >> 16))) * a.norm;
+        if (cur.live) {
+            const uint32_t sy[4] = {cur.sy.x, cur.sy.y, cur.sy.z, cur.sy.w};
+            const float sc = __half2float(__ushort_as_half((unsigned short)(cur.meta.x & 0xffffu))) * a.norm;
+            const float zr = __half2float(__ushort_as_half((unsigned short)(cur.meta.x >> 16))) * a.norm;
             const uint32_t al =
-                __float_as_uint(__half2float(__ushort_as_half((unsigned short)(m.y & 0xffffu))) * a.norm);
+                __float_as_uint(__half2float(__ushort_as_half((unsigned short)(cur.meta.y & 0xffffu))) * a.norm);
             const float2 sc2 = make_float2(sc, sc), zr2 = make_float2(zr, zr);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const uint32_t off = ~(sy[c] >> (8 * g));  // bit i set: s = -1
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 cen = mytab[((cw[c] >> (8 * j)) & 0xffu) * 16];
+                    const float2 cen = mytab[((cur.cw[c] >> (8 * j)) & 0xffu) * 16];
                     const float2 s = make_float2(__uint_as_float(al ^ ((off << (31 - 2 * j)) & 0x80000000u)),
                                                  __uint_as_float(al ^ ((off << (30 - 2 * j)) & 0x80000000u)));
                     P[c][j] = add2(__ffma2_rn(cen, sc2, zr2), s);
@@ -155,7 +169,7 @@ __global__ void __launch_bounds__(kReadWarps * 32, 3) dequant_paged_kernel(const
             }
         }
         if (valid) {
-            __half *dst = jb.out + (int64_t)v * kD + 8 * g;
+            __half *dst = out + (int64_t)v * kD + 8 * g;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t w[4];

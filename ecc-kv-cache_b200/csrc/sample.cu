@@ -102,24 +102,7 @@ struct Bins {
     uint32_t count[kBins];
     unsigned long long mass[kBins];
 };
-constexpr int kList = sizeof(Shared::hist) / 8;
 static_assert(sizeof(Bins) <= sizeof(Shared::hist), "room for the bins");
-
-// Descending sort of the first power of two >= n entries (those from n on must
-// be zero) of `x` by the whole block.
-__device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
-    int size = 1;
-    while (size < n) size *= 2;
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int i = 2 * t - (t & (j - 1));  // bit j of i is clear
-                const unsigned long long p = x[i], q = x[i + j];
-                if ((p < q) == ((i & k) == 0)) x[i] = q, x[i + j] = p;
-            }
-            __syncthreads();
-        }
-}
 
 // w * 2^S as an integer.
 struct Mass {
