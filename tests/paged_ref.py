@@ -62,8 +62,10 @@ def attend(q, k_pool, v_pool, table, lens, window=0, sinks=0, rotate=False):
 
     Bounds (u = 2^-11, half a step of fp16; w = 2^-22):
     * a score: the tensor-core sum of 128 products (hi + lo parts carry a level to w relative, eight chained steps each
-      lose at most w of the magnitudes added), so 12 w sm sum |q| (|C| scale + 2 alpha + |zero|), plus w |s|; with the
-      query rotated inside, its rounding to fp16 adds u sm sum |q||k|;
+      lose at most w of the magnitudes added), so 12 w sm sum |q| (|C| scale + 2 alpha + |zero|), plus w |s|; a query
+      rotated inside is carried to 2^-14 at least (fp16 and a remainder of three bits), which adds u/8 sm sum |q||k|;
+    * the values' centroids are carried as one fp16 each (of the level times a factor chosen for it): 8.6e-5 of
+      |C| scale at most;
     * a probability: twice the largest score error, plus the 2^-21 of two base-2 exponentials, relative;
     * an output: the probabilities' error times sum p |v|, the fp16 sign weights u alpha, 16 w of the sums, and u |out|
       for the last rounding; the inverse rotation adds up the bounds of 128 elements over sqrt(128)."""
@@ -89,7 +91,7 @@ def attend(q, k_pool, v_pool, table, lens, window=0, sinks=0, rotate=False):
                 s = SM * (k @ x)
                 e = 12 * w * SM * (size @ np.abs(x)) + w * np.abs(s)
                 if rotate:
-                    e = e + u * SM * (np.abs(k) @ np.abs(x))
+                    e = e + u / 8 * SM * (np.abs(k) @ np.abs(x))
                 e = e.max()
                 m = s.max()
                 p = np.exp(s - m)
@@ -101,6 +103,8 @@ def attend(q, k_pool, v_pool, table, lens, window=0, sinks=0, rotate=False):
                 w_tol[b, h, t] += p * (rel + 4 * w) + 2.0 ** -40
                 o = p @ v
                 d = rel * (p @ np.abs(v)) + u * (p @ alpha) + 16 * w * (p @ np.abs(v)) + 1e-7
+                vc, _, vm = fields(vb)
+                d = d + 8.6e-5 * (p @ (np.abs(vc) * vm[:, 0:1]))
                 if rotate:
                     o, d = o @ H, np.full(128, d.sum() / np.sqrt(128.0))
                 out[b, h * G + g], tol[b, h * G + g] = o, d + u * np.abs(o) + 2.0 ** -25
