@@ -6,6 +6,7 @@ from typing import Generator, Optional
 import torch
 
 from .cache import ErrorCorrectedCache
+from .paged import PagedErrorCorrectedCache
 from .patch import patch_model, unpatch_model
 
 
@@ -24,6 +25,28 @@ def ecc_cache(model, batch_size: int = 1, max_cache_len: int = 128_000, device: 
     """
     cache = ErrorCorrectedCache(config=model.config, batch_size=batch_size, max_cache_len=max_cache_len,
                                 device=device, **cache_kwargs)
+    patch_model(model, cache)
+    try:
+        yield cache
+    finally:
+        unpatch_model()
+        del cache
+        if torch.cuda.is_available():
+            torch.cuda.empty_cache()
+
+
+@contextmanager
+def paged_ecc_cache(model, batch_size: int = 1, max_cache_len: int = 32768, device: Optional[str] = None,
+                    **cache_kwargs) -> Generator[PagedErrorCorrectedCache, None, None]:
+    """``ecc_cache`` with a PagedErrorCorrectedCache: sequences of different
+    lengths, a sliding window with sinks, eviction by attention weight.
+
+        with paged_ecc_cache(model, batch_size=8, collect_weights=True) as cache:
+            ...
+            cache.evict(budget=4096, sinks=4, recent=512)
+    """
+    cache = PagedErrorCorrectedCache(config=model.config, batch_size=batch_size, max_cache_len=max_cache_len,
+                                     device=device, **cache_kwargs)
     patch_model(model, cache)
     try:
         yield cache
