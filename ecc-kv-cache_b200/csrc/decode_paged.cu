@@ -49,7 +49,6 @@ struct DecodeArgs {
     int window, sinks;
     float scale_log2;
     int flags;
-    bool halves;  // a stage is fetched as two 16-token boxes (pages that are no multiple of 32 tokens)
     float *pm, *pl, *po;
     int *row_first, *row_last;  // first and last range of a row
     float *raw;                 // log2-scaled scores [row][capacity][G], or null
@@ -110,7 +109,10 @@ struct Cursor {
     SeqTiles st;
 };
 
-template <int G, bool kScores>
+// kHalves: a stage is fetched as two 16-token boxes by two lanes, for pages that
+// are no multiple of 32 tokens.  (A form of its own: with one box a stage every
+// cursor is the same in all lanes, which the other form's loop pays 4 % for.)
+template <int G, bool kScores, bool kHalves>
 __global__ void __launch_bounds__(kThreads, 1)
 decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_constant__ CUtensorMap mks,
                     const __grid_constant__ CUtensorMap mvc, const __grid_constant__ CUtensorMap mvs,
@@ -206,13 +208,13 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     const int *p_row;  // the sequence's row of the table
     auto page_at = [&](int pi) { return pi < a.t.width ? __ldg(p_row + pi) : -1; };
     auto start_run = [&]() {
-        const int tb = prod.st.base(prod.u) + (a.halves ? 16 * (lane & 1) : 0);
+        const int tb = prod.st.base(prod.u) + (kHalves ? 16 * (lane & 1) : 0);
         p_left = (prod.u < prod.st.nsink ? prod.st.nsink : prod.st.n) - prod.u;
         p_row = a.t.table + (int64_t)prod.b * a.t.stride;
         p_pi = (int)a.t.page_of(tb);
         p_slot = tb - p_pi * a.t.page_size;
         p_page = page_at(p_pi);
-        if (!a.halves) p_next = page_at(p_pi + 1);
+        if (!kHalves) p_next = page_at(p_pi + 1);
     };
     auto issue_next = [&](int s, bool more) {
         const uint32_t bar = bars + 8 * s;
@@ -220,8 +222,8 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             fence_proxy_async();  // this warp's earlier reads of the stage precede the overwrite
             mbar_expect_tx(bar, kStageBytes);
         }
-        if (a.halves) __syncwarp();
-        if (lane == 0 || (lane == 1 && a.halves)) {
+        if (kHalves) __syncwarp();
+        if (lane == 0 || (kHalves && lane == 1)) {
             int page = p_page;
             if ((uint32_t)page >= (uint32_t)a.t.n_pages) {
                 // no such page: the copy reads zeros out of the map's range.  The second half of
@@ -230,7 +232,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
                 page = a.t.n_pages;
             }
             const uint32_t dst = ring + s * kStageBytes;
-            if (a.halves) fence_proxy_async();
+            if (kHalves) fence_proxy_async();
             tma_4d(dst + kOffKC + lane * kSubC, &mkc, 0, p_slot, prod.h, page, bar);
             tma_4d(dst + kOffKS + lane * kSubS, &mks, 64, p_slot, prod.h, page, bar);
             tma_4d(dst + kOffVC + lane * kSubC, &mvc, 0, p_slot, prod.h, page, bar);
@@ -241,7 +243,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         if (--p_left == 0) {
             if (prod.u == prod.st.n) advance_row(prod);
             start_run();
-        } else if (a.halves) {
+        } else if (kHalves) {
             p_slot += kTile;
             if (p_slot >= a.t.page_size) {  // by one or two pages
                 do {
@@ -567,21 +569,28 @@ static int check_shape(int B, int Hq, int Hkv, int64_t capacity) {
     return ECC_OK;
 }
 
-template <int G, bool kScores>
-static int launch(const CUtensorMap (&m)[4], const DecodeArgs &a, int grid, cudaStream_t s) {
+template <int G, bool kScores, bool kHalves>
+static int launch_form(const CUtensorMap (&m)[4], const DecodeArgs &a, int grid, cudaStream_t s) {
     static bool configured[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ECC_ERR_DEVICE;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        if (cudaFuncSetAttribute(decode_paged_kernel<G, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        if (cudaFuncSetAttribute(decode_paged_kernel<G, kScores, kHalves>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kSmPaged) != cudaSuccess)
             return ECC_ERR_CUDA;
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    if (launch_pdl(decode_paged_kernel<G, kScores>, dim3(grid), dim3(kThreads), kSmPaged, s, m[0], m[1], m[2], m[3],
+    if (launch_pdl(decode_paged_kernel<G, kScores, kHalves>, dim3(grid), dim3(kThreads), kSmPaged, s, m[0], m[1], m[2], m[3],
                    a) != cudaSuccess)
         return ECC_ERR_LAUNCH;
     return launch_status();
+}
+
+template <int G>
+static int launch(const CUtensorMap (&m)[4], const DecodeArgs &a, int grid, bool halves, cudaStream_t s) {
+    if (a.raw)
+        return halves ? launch_form<G, true, true>(m, a, grid, s) : launch_form<G, true, false>(m, a, grid, s);
+    return halves ? launch_form<G, false, true>(m, a, grid, s) : launch_form<G, false, false>(m, a, grid, s);
 }
 
 template <int G>
@@ -662,7 +671,7 @@ extern "C" int ecc_decode_paged(const void *q_f16, const void *k_blocks, const v
     a.sinks = sinks;
     a.scale_log2 = (sm_scale > 0.0f ? sm_scale : 1.0f / std::sqrt((float)kD)) * 1.4426950408889634f;
     a.flags = flags;
-    a.halves = a.t.width > 1 && a.t.page_size % kTile != 0;
+    const bool halves = a.t.width > 1 && a.t.page_size % kTile != 0;
     a.pm = reinterpret_cast<float *>(w + l.pm);
     a.pl = reinterpret_cast<float *>(w + l.pl);
     a.po = reinterpret_cast<float *>(w + l.po);
@@ -674,13 +683,13 @@ extern "C" int ecc_decode_paged(const void *q_f16, const void *k_blocks, const v
 
     CUtensorMap m[4];
     if (make_maps(&m[0], &m[1], &m[2], &m[3], k_blocks, v_blocks, a.t.page_size, Hkv, a.t.n_pages, bs_h, bs_p, rb,
-                  a.halves ? 16 : kTile) != ECC_OK)
+                  halves ? 16 : kTile) != ECC_OK)
         return ECC_ERR_ALIGN;  // strides a tensor map cannot describe
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int G = Hq / Hkv;
     switch (G) {
 #define ECC_PAGED_CASE(N) \
-    case N: rc = weights ? launch<N, true>(m, a, l.grid, s) : launch<N, false>(m, a, l.grid, s); break;
+    case N: rc = launch<N>(m, a, l.grid, halves, s); break;
         ECC_PAGED_CASE(1) ECC_PAGED_CASE(2) ECC_PAGED_CASE(3) ECC_PAGED_CASE(4)
         ECC_PAGED_CASE(5) ECC_PAGED_CASE(6) ECC_PAGED_CASE(7) ECC_PAGED_CASE(8)
 #undef ECC_PAGED_CASE

@@ -1050,8 +1050,12 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     heads, is added to it in place.  ``return_lse``: also the natural log of
     each row's sum of e^score, [B, Hq] fp32.  A sequence of length 0 gives a
     zero row (lse -inf) and adds no weight.  GQA groups of up to 8."""
-    q3 = _query(query)
-    B, hq, _ = q3.shape
+    _require_cuda(query, "query")
+    qs = query.shape
+    if query.dtype is not torch.float16 or len(qs) not in (3, 4) or qs[-1] != D or (len(qs) == 4 and qs[2] != 1):
+        raise RuntimeError("query must be float16 [B, Hq, 1, 128] (or [B, Hq, 128]): one token per sequence")
+    q3 = query if query.is_contiguous() else query.contiguous()
+    B, hq = qs[0], qs[1]
     shape, ks, vs = _paged_pools(k_pool, v_pool)
     if ks != vs:
         raise RuntimeError("k_pool and v_pool must have the same strides")
@@ -1067,7 +1071,7 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     capacity = pages.width * pages.page_size
     wp, wb, wh = (None, 0, 0) if weights is None else _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out is None:
-        out = torch.empty((B, hq, 1, D), dtype=torch.float16, device=dev)
+        out = torch.empty_like(q3) if len(qs) == 4 else torch.empty((B, hq, 1, D), dtype=torch.float16, device=dev)
     elif not out.is_contiguous() or out.dtype is not torch.float16 or out.numel() != B * hq * D or out.device != dev:
         raise RuntimeError("out must be a contiguous float16 tensor of B*Hq*128 elements on the pools' device")
     lse = torch.empty((B, hq), dtype=torch.float32, device=dev) if return_lse else None
