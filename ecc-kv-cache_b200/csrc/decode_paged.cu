@@ -489,10 +489,12 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
 }
 
 // weights[b, h, t] += sum over the group's heads of 2^(score - lse) for the
-// visible tokens: one thread per token, the kept scores of a token are
-// contiguous.  Bound by memory: 4 G bytes of scores and 8 bytes of weights a
-// token.
+// visible tokens: a thread per token, kWeightTake tiles of a warp in flight,
+// the kept scores of a token are contiguous.  Bound by memory: 4 G bytes of
+// scores and 8 bytes of weights a token.
 constexpr int kWeightThreads = 256;
+constexpr int kWeightTake = 4;
+constexpr int kWeightTiles = kWeightTake * kWeightThreads / 32;  // per CTA and step
 template <int G>
 __global__ void __launch_bounds__(kWeightThreads)
 paged_weights_kernel(const __grid_constant__ DecodeArgs a, const float *__restrict__ lse2, float *__restrict__ weights,
@@ -505,27 +507,40 @@ paged_weights_kernel(const __grid_constant__ DecodeArgs a, const float *__restri
         const int row = (int)(item / chunks), chunk = (int)(item - (int64_t)row * chunks);
         const int b = row / a.Hkv, h = row - b * a.Hkv;
         const SeqTiles st(seq_len_of(a, b), a.window, a.sinks);
-        const int u = chunk * (kWeightThreads / 32) + warp;
-        if (u >= st.n) continue;
-        const int tb = st.base(u);
-        if (!((st.visible(tb, a.sinks) >> lane) & 1u)) continue;
-        const float *s = a.raw + ((int64_t)row * a.t.capacity + tb + lane) * G;
-        float x[G];
-        if constexpr (G % 4 == 0) {
+        const int u0 = chunk * kWeightTiles + warp * kWeightTake;
+        if (u0 >= st.n) continue;
+        float l2[G];
 #pragma unroll
-            for (int k = 0; k < G; k += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(s + k);
-                x[k] = v.x, x[k + 1] = v.y, x[k + 2] = v.z, x[k + 3] = v.w;
+        for (int k = 0; k < G; ++k) l2[k] = __ldg(lse2 + (int64_t)row * G + k);
+        float x[kWeightTake][G], old[kWeightTake];
+        float *w[kWeightTake];
+#pragma unroll
+        for (int j = 0; j < kWeightTake; ++j) {
+            const int tb = st.base(u0 + j);
+            w[j] = nullptr;
+            if (u0 + j >= st.n || !((st.visible(tb, a.sinks) >> lane) & 1u)) continue;
+            w[j] = weights + b * ws_b + h * ws_h + tb + lane;
+            const float *s = a.raw + ((int64_t)row * a.t.capacity + tb + lane) * G;
+            if constexpr (G % 4 == 0) {
+#pragma unroll
+                for (int k = 0; k < G; k += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(s + k);
+                    x[j][k] = v.x, x[j][k + 1] = v.y, x[j][k + 2] = v.z, x[j][k + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < G; ++k) x[j][k] = s[k];
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < G; ++k) x[k] = s[k];
+            old[j] = *w[j];
         }
-        float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < G; ++k) sum += exp2f(x[k] - __ldg(lse2 + (int64_t)row * G + k));
-        float *w = weights + b * ws_b + h * ws_h + tb + lane;
-        *w += sum;
+        for (int j = 0; j < kWeightTake; ++j) {
+            if (!w[j]) continue;
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < G; ++k) sum += exp2f(x[j][k] - l2[k]);
+            *w[j] = old[j] + sum;
+        }
     }
 }
 
@@ -596,9 +611,8 @@ static int launch(const CUtensorMap (&m)[4], const DecodeArgs &a, int grid, bool
 template <int G>
 static int launch_weights(const DecodeArgs &a, const float *lse2, float *w, int64_t ws_b, int64_t ws_h,
                           cudaStream_t s) {
-    const int per = kWeightThreads / 32;
     const int tiles = (a.t.capacity + kTile - 1) / kTile;
-    const int chunks = (tiles + per - 1) / per;
+    const int chunks = (tiles + kWeightTiles - 1) / kWeightTiles;
     const int64_t items = (int64_t)a.B * a.Hkv * chunks;
     const int64_t grid = std::min<int64_t>(items, (int64_t)sm_count() * 8);
     if (launch_pdl(paged_weights_kernel<G>, dim3((unsigned)grid), dim3(kWeightThreads), 0, s, a, lse2, w, ws_b, ws_h,

@@ -40,6 +40,10 @@ struct EvictArgs {
 // Weight -> key: NaN above everything, as a sort has it.
 __device__ __forceinline__ uint32_t weight_key(float x) { return x != x ? 0xffffffffu : sel::key_of(x); }
 
+__device__ __forceinline__ float key_weight(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);  // the NaN key gives a NaN
+}
+
 __device__ void check_tables(const EvictArgs &a, sel::cg::cluster_group &cl) {
     const int t0 = cl.block_rank() * sel::kThreads + threadIdx.x, step = cl.num_blocks() * sel::kThreads;
     for (int i = t0; i < (a.src.n_pages + 31) / 32; i += step) a.bitmap[i] = 0;
@@ -92,10 +96,11 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
         if (i < a.budget) kept[i] = -1;
         if (i < a.ow_len) ow[i] = 0.0f;
     }
-    auto put = [&](int i, int t) {
+    auto put_as = [&](int i, int t, float x) {
         kept[i] = t;
-        if (i < a.ow_len) ow[i] = w[t];
+        if (i < a.ow_len) ow[i] = x;
     };
+    auto put = [&](int i, int t) { put_as(i, t, w[t]); };
     if (L <= a.budget) {  // cluster-uniform
         for (int i = rank * sel::kThreads + tid; i < L; i += C * sel::kThreads) put(i, i);
         return;
@@ -111,7 +116,8 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
     const int base = a.sinks + min(n_all, rank * per), n = min(n_all, (rank + 1) * per) - min(n_all, rank * per);
     const bool cached = n <= a.cache_keys;
     if (cached) {
-        for (int i = tid; i < n; i += sel::kThreads) cache[i] = weight_key(w[base + i]);
+#pragma unroll 8
+        for (int i = tid; i < n; i += sel::kThreads) cache[i] = weight_key(__ldg(w + base + i));
         __syncthreads();
     }
     auto key = [&](int i) { return cached ? cache[i] : weight_key(__ldg(w + base + i)); };
@@ -174,10 +180,13 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
     int lo, hi;
     sel::warp_part(n, lo, hi);
     uint32_t at = a.sinks + sel::cluster_exclusive(sh, cl, sel::warp_count(lo, hi, keep));
+#pragma unroll 4
     for (int i0 = lo; i0 < hi; i0 += 32) {
         const bool hit = i0 + lane < hi && keep(i0 + lane);
         const uint32_t m = __ballot_sync(0xffffffffu, hit);
-        if (hit) put((int)(at + __popc(m & ((1u << lane) - 1u))), base + i0 + lane);
+        const int to = (int)(at + __popc(m & ((1u << lane) - 1u))), t = base + i0 + lane;
+        // the weight again out of its key (-0 comes back as +0)
+        if (hit) put_as(to, t, cached ? key_weight(cache[i0 + lane]) : __ldg(w + t));
         at += __popc(m);
     }
 }

@@ -156,6 +156,25 @@ __device__ __forceinline__ uint64_t cluster_sum(Shared &sh, cg::cluster_group &c
     return all;
 }
 
+// Two sums at once: a pair per CTA in the first CTAs' entries of `share`.
+__device__ __forceinline__ ulonglong2 cluster_sum2(Shared &sh, cg::cluster_group &cl, uint64_t x, uint64_t y) {
+    static_assert(kMaxCluster >= 16, "two entries for each of 8 CTAs");
+    const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    uint64_t ax, ay;
+    block_exclusive(x, sh.warp64, &ax);
+    block_exclusive(y, sh.warp64, &ay);
+    if (threadIdx.x < ranks) {
+        uint64_t *to = of_rank(cl, sh.cross.share, threadIdx.x);
+        to[2 * rank] = ax;
+        to[2 * rank + 1] = ay;
+    }
+    cl.sync();
+    ulonglong2 s = make_ulonglong2(0, 0);
+    for (int r = 0; r < ranks; ++r) s.x += sh.cross.share[2 * r], s.y += sh.cross.share[2 * r + 1];
+    cl.sync();  // share may be written again
+    return s;
+}
+
 // The top-p threshold inside a bin of many (nearly) equal logits, by the bits
 // of their keys: a descent like kth_largest's whose digits are found by mass.
 // Returns the new threshold key and cut.
@@ -366,12 +385,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             uint32_t at = 0;
             if (lane == 0) at = atomicAdd(of_rank(cl, &wk.listed, 0), (uint32_t)__popc(m));
             at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
-            if (hit) of_rank(cl, list, 0)[at] = ((unsigned long long)kx << 32) | (uint32_t)~(uint32_t)(base + i);
+            if (hit && at < kList) of_rank(cl, list, 0)[at] = ((unsigned long long)kx << 32) | (uint32_t)~(uint32_t)(base + i);
         };
         // Waits for the list and sorts it in rank 0, descending.  Returns its length.
         auto sorted = [&]() {
             cl.sync();
-            const int m = wk.listed;
+            const int m = min((int)wk.listed, kList);
             if (rank == 0) {
                 int size = 1;
                 while (size < m) size *= 2;
@@ -493,11 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             cl.sync();  // every CTA has its copy; the second search starts from the same sums
             const Crossing to = crossing(sh.cross, cl, wk.tot_mass, min(aim + slack, about), sh.warp64);
             const int b0 = (int)from.slot, b1 = aim + slack < about ? (int)to.slot : kBins - 1;
-            // tokens in b0 .. b1
-            uint32_t near = 0;
-            for (int i = tid; i < W; i += kThreads)
-                near += rank * W + i >= b0 && rank * W + i <= b1 ? wk.tot_count[i] : 0;
-            if (cluster_sum(sh, cl, near) <= kList) {
+            {
                 const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
                 int lo, hi;
                 warp_part(n, lo, hi);
@@ -527,8 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
                 if (lane == 0) wk.part[warp] = part;
-                const uint64_t want = want_of(cluster_sum(sh, cl, all));
-                above = cluster_sum(sh, cl, above);
+                const ulonglong2 sums = cluster_sum2(sh, cl, all, above);
+                const uint64_t want = want_of(sums.x);
+                above = sums.y;
                 const int m = sorted();
                 if (rank == 0) {
                     if (tid == 0) for (int r = 0; r < C; ++r) *of_rank(cl, &wk.kth, r) = 0;
@@ -540,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                         const uint64_t w = i < m ? listed_mass(i) : 0;
                         uint64_t sum;
                         const uint64_t mine = before + block_exclusive(w, sh.warp64, &sum);
-                        if (i < m && mine < want) {
+                        if (i < m && mine < want && wk.listed <= kList) {
                             if (want <= mine + w) publish(list[i]);
                             if (w >= least) {
                                 const int at = (int)~(uint32_t)list[i], r = at / a.slice;
@@ -553,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 }
                 take();
                 parts_known = kth != 0;  // no key is 0
-                if (!parts_known) cut = 0xffffffffu;  // the end was not in the list: the exact search below
+                if (!parts_known) cut = 0xffffffffu;  // the list was too short: the exact search below
             }
         }
         if (by_mass && !parts_known) count_bins(std::integral_constant<int, kMassToo>());
