@@ -17,6 +17,7 @@ path, and CPU tensors raise ``RuntimeError`` like the reference's
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import threading
@@ -882,11 +883,12 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 # ---------------------------------------------------------------------------
 def _launch(fn, what: str, dev: torch.device, *args) -> None:
     """fn(*args, current stream of dev) with dev the current device."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    i = dev.index
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         _check(rc, what)
 
@@ -900,16 +902,13 @@ def _scratch(workspace: torch.Tensor | None, dev: torch.device, need: int) -> to
                 or workspace.numel() * workspace.element_size() < need:
             raise RuntimeError(f"workspace must be contiguous, on the pools' device and hold {need} bytes")
         return workspace
-    with_dev = torch.cuda.current_device() == dev.index
-    if with_dev and not torch.cuda.is_current_stream_capturing():
-        ws = _ws_cache.get((dev.index, torch._C._cuda_getCurrentRawStream(dev.index)))
-        if ws is not None and ws.numel() >= need:
-            return ws
-        return _workspace(dev, need)
-    with torch.cuda.device(dev):
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(need, dtype=torch.uint8, device=dev)
-        return _workspace(dev, need)
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _scratch(None, dev, need)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = _ws_cache.get((dev.index, torch._C._cuda_getCurrentRawStream(dev.index)))
+    return ws if ws is not None and ws.numel() >= need else _workspace(dev, need)
 
 
 def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None):
@@ -919,33 +918,38 @@ def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None):
     shape = k_pool.shape
     if k_pool.dtype is not torch.uint8 or len(shape) != 4 or shape[3] not in (BLOCK_BYTES, RECORD96):
         raise RuntimeError("k_pool must be a uint8 pool [pages, Hkv, page_size, 128] (or [.., 96])")
-    strides = []
-    for t, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-        if t is None:
-            strides.append((0, 0))
-            continue
-        if t is not k_pool:
-            _require_cuda(t, name)
-            if t.shape != shape or t.dtype is not torch.uint8 or t.device != k_pool.device:
-                raise RuntimeError("k_pool and v_pool must have the same shape, type and device")
-        sp, sh, st, s1 = t.stride()
-        rb = shape[3]
-        if s1 != 1 or st != rb or sp % rb or sh % rb:
-            raise RuntimeError(f"{name}: a page's blocks must be contiguous {rb}-byte rows, page and head strides whole "
-                               f"blocks")
-        strides.append((sp // rb, sh // rb))
-    return shape, strides[0], strides[1]
+    rb = shape[3]
+    strides = k_pool.stride()
+    sp, sh, st, s1 = strides
+    if s1 != 1 or st != rb or sp % rb or sh % rb:
+        raise RuntimeError(f"k_pool: a page's blocks must be contiguous {rb}-byte rows, page and head strides whole blocks")
+    ks = vs = (sp // rb, sh // rb)
+    if v_pool is not None:
+        _require_cuda(v_pool, "v_pool")
+        if v_pool.shape != shape or v_pool.dtype is not torch.uint8 or v_pool.device != k_pool.device:
+            raise RuntimeError("k_pool and v_pool must have the same shape, type and device")
+        if v_pool.stride() != strides:
+            sp, sh, st, s1 = v_pool.stride()
+            if s1 != 1 or st != rb or sp % rb or sh % rb:
+                raise RuntimeError(f"v_pool: a page's blocks must be contiguous {rb}-byte rows, page and head strides whole "
+                                   f"blocks")
+            vs = (sp // rb, sh // rb)
+    return shape, ks, vs
 
 
 def _pages(table: torch.Tensor, name: str, B: int, shape, dev: torch.device) -> _Pages:
     if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.device != dev:
         raise RuntimeError(f"{name} must be an int32 tensor on the pools' device")
-    if table.dim() != 2 or table.shape[0] != B or table.shape[1] < 1 or table.stride(1) != 1:
-        raise RuntimeError(f"{name} must be int32 [B, width] with contiguous rows, one row per sequence")
-    width = table.shape[1]
+    ts = table.shape
+    if len(ts) != 2 or ts[0] != B or ts[1] < 1:
+        raise RuntimeError(f"{name} must be int32 [B, width], one row per sequence")
+    width = ts[1]
+    row, col = table.stride()
+    if col != 1:
+        raise RuntimeError(f"{name} must have contiguous rows")
     if shape[2] % 16 and width > 1:
         raise RuntimeError(f"page_size must be a multiple of 16 (or one page per sequence), got {shape[2]}")
-    return _Pages(table.data_ptr(), table.stride(0), width, shape[2], shape[0])
+    return _Pages(table.data_ptr(), row, width, shape[2], shape[0])
 
 
 def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> int:
@@ -1028,6 +1032,11 @@ def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_ta
     return out if n == 2 else out[0]
 
 
+@functools.lru_cache(1024)
+def _decode_paged_bytes(B: int, hq: int, hkv: int, capacity: int, with_weights: bool, device: int) -> int:
+    return int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(with_weights)))
+
+
 def decode_paged_workspace_size(B: int, hq: int, hkv: int, capacity: int, with_weights: bool = False) -> int:
     """Workspace bytes of decode_attention_paged for tables that can name
     ``capacity`` = width * page_size tokens."""
@@ -1076,7 +1085,7 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
         raise RuntimeError("out must be a contiguous float16 tensor of B*Hq*128 elements on the pools' device")
     lse = torch.empty((B, hq), dtype=torch.float32, device=dev) if return_lse else None
     flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | (BLOCK96 if shape[3] == RECORD96 else 0)
-    ws = _scratch(workspace, dev, _lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, weights is not None))
+    ws = _scratch(workspace, dev, _decode_paged_bytes(B, hq, hkv, capacity, weights is not None, dev.index))
     _launch(_lib.ecc_decode_paged, "decode_attention_paged", dev, q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
             ks[0], ks[1], pages, lens, out.data_ptr(), None if lse is None else lse.data_ptr(), wp, wb, wh, ws.data_ptr(),
             ws.numel() * ws.element_size(), B, hq, hkv, 0.0 if sm_scale is None else float(sm_scale), int(window),
@@ -1119,7 +1128,7 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     capacity = pages.width * pages.page_size
     wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out_weights is None:
-        out_weights = torch.empty((B, hkv, weights.shape[2]), dtype=torch.float32, device=dev)
+        out_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
     op, ob, oh = _weights_like(out_weights, "out_weights", B, hkv, capacity, dev)
     if out_weights.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
         raise RuntimeError("out_weights must not share memory with weights")
