@@ -259,7 +259,10 @@ __device__ __forceinline__ bool paged_dst(const PagedJobs &jobs, const CompressJ
     const int64_t L = jb.div_l.d;
     if (jobs.new_lens) {
         const int n = __ldg(jobs.new_lens + b);
-        if (n < 0 || n > L) atomicExch(&paged::g_paged_error, 5);
+        if (n < 0 || n > L) {
+            atomicExch(&paged::g_paged_error, 5);
+            return false;
+        }
         if (l >= n) return false;
     }
     const int64_t p = (int64_t)__ldg(jobs.pos + b) + l;

@@ -967,6 +967,11 @@ def _weights_like(t: torch.Tensor, name: str, B: int, hkv: int, capacity: int, d
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to its last."""
+    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else 0
+
+
 def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
                         block_table: torch.Tensor, pos: torch.Tensor, new_lens: torch.Tensor | None = None,
                         rotate: bool = True) -> None:
@@ -1034,7 +1039,8 @@ def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_ta
 
 @functools.lru_cache(1024)
 def _decode_paged_bytes(B: int, hq: int, hkv: int, capacity: int, with_weights: bool, device: int) -> int:
-    return int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(with_weights)))
+    with torch.cuda.device(device):  # the partial slots follow the device's SMs
+        return int(_lib.ecc_decode_paged_workspace_size(B, hq, hkv, capacity, int(with_weights)))
 
 
 def decode_paged_workspace_size(B: int, hq: int, hkv: int, capacity: int, with_weights: bool = False) -> int:
@@ -1088,8 +1094,8 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     ws = _scratch(workspace, dev, _decode_paged_bytes(B, hq, hkv, capacity, weights is not None, dev.index))
     _launch(_lib.ecc_decode_paged, "decode_attention_paged", dev, q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
             ks[0], ks[1], pages, lens, out.data_ptr(), None if lse is None else lse.data_ptr(), wp, wb, wh, ws.data_ptr(),
-            ws.numel() * ws.element_size(), B, hq, hkv, 0.0 if sm_scale is None else float(sm_scale), int(window),
-            int(sinks), flags)
+            ws.numel() * ws.element_size(), B, hq, hkv, 0.0 if sm_scale is None else float(sm_scale),
+            min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff), flags)
     return (out, lse) if return_lse else out
 
 
@@ -1130,7 +1136,7 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     if out_weights is None:
         out_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
     op, ob, oh = _weights_like(out_weights, "out_weights", B, hkv, capacity, dev)
-    if out_weights.untyped_storage().data_ptr() == weights.untyped_storage().data_ptr():
+    if op < wp + _span(weights) and wp < op + _span(out_weights):
         raise RuntimeError("out_weights must not share memory with weights")
     if kept is None:
         kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)

@@ -152,11 +152,14 @@ def test_evict_refusals():
     table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
     out = table + 8
     w, n = torch.zeros(2, 2, 64, device="cuda"), i32([64, 64])
+    wide = torch.zeros(2, 2, 96, device="cuda")
     args = dict(k_pool=pool, v_pool=pool.clone(), block_table=table, seq_lens=n, weights=w, out_table=out, budget=40)
     ops.evict_paged(**args)
+    both = torch.zeros(2, 2, 2, 64, device="cuda")  # two halves of one tensor are two tensors
+    ops.evict_paged(**{**args, "weights": both[0], "out_weights": both[1]})
     for b in (dict(budget=0), dict(budget=65), dict(sinks=-1), dict(recent=-1), dict(sinks=30, recent=11),
               dict(out_table=table), dict(out_table=out[:1]), dict(out_table=out.long()), dict(weights=w.half()),
-              dict(weights=w[..., :63]), dict(weights=w[:1]), dict(out_weights=w), dict(seq_lens=n[:1]),
+              dict(weights=w[..., :63]), dict(weights=w[:1]), dict(out_weights=w), dict(weights=wide[:, :, :64], out_weights=wide[:, :, 32:96]), dict(seq_lens=n[:1]),
               dict(kept=torch.zeros(2, 2, 39, dtype=torch.int32, device="cuda")), dict(k_pool=pool[..., :96]),
               dict(workspace=torch.zeros(4, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(RuntimeError):

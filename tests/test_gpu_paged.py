@@ -280,6 +280,37 @@ def test_append_out_of_range_writes_nothing(L):
         ops.compress_pair_paged(x, x, pool, pool.clone(), t, i32(pos), new_lens=None if new is None else i32(new))
         assert ops.device_status(reset=True) == 5
         assert int(pool.max()) == 0
+    one = pool.clone()
+    ops.compress_pair_paged(x, None, one, None, table, i32([0, 0]), new_lens=i32([L + 1, 1]))  # the other goes on
+    assert ops.device_status(reset=True) == 5
+    assert not one[:200].any() and one[200, :, 0].any() and not one[200, :, 1:].any()
+
+
+def test_pages_beyond_four_gigabytes():
+    """Append, read-back, decode and eviction on pages whose byte offsets pass 32 bits."""
+    import custom_ecc_cuda as ops
+    hkv, ps = 4, 256
+    per = hkv * ps * 128
+    total = (1 << 32) // per + 40
+    g = torch.Generator(device="cuda").manual_seed(0)
+    big = [torch.empty(total, hkv, ps, 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    small = [torch.empty(8, hkv, ps, 128, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    far = torch.tensor([[total - 1, total - 7, 3]], dtype=torch.int32, device="cuda")
+    near = torch.tensor([[5, 1, 3]], dtype=torch.int32, device="cuda")
+    x = [torch.randn(1, hkv, 700, 128, generator=g, device="cuda").half() for _ in range(2)]
+    q = torch.randn(1, 8, 1, 128, generator=g, device="cuda").half()
+    got = []
+    for pools, table, out in ((big, far, far - 1), (small, near, near - 1)):
+        ops.compress_pair_paged(x[0], x[1], *pools, table, i32([0]))
+        w = torch.zeros(1, hkv, 768, device="cuda")
+        o = ops.decode_attention_paged(q, *pools, table, i32([700]), weights=w)
+        k, v = ops.dequantize_paged(*pools, table, i32([700]), 700)
+        ow, kept = ops.evict_paged(*pools, table, i32([700]), w, out, 400, sinks=3, recent=50)
+        ek, ev = ops.dequantize_paged(*pools, out, i32([400]), 400)
+        got.append((o, w, k, v, ow, kept, ek, ev))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert (got[0][2] - x[0]).float().norm() < 0.2 * x[0].float().norm()
 
 
 def test_append_refusals():
