@@ -20,6 +20,13 @@
 // along the tiles w or r grows by one at every new (range, row) pair, so the
 // slots are distinct, a row's slots are contiguous, and NW + rows slots
 // suffice for every distribution of lengths.  paged_merge_kernel joins them.
+//
+// Measured at 8 sequences x 65531 tokens, 32 query and 8 kv heads, pages of 128
+// tokens (1.07 GB of blocks): 223 us with the merge, 4.8 TB/s; the loads alone
+// take 169 us and the arithmetic alone 212.  It is bound by the latency of
+// dependent instructions at three warps of 168 registers per scheduler (ncu:
+// issue 56 %, shared-memory wavefronts 60 %, ALU 50 %, tensor 36 %), and in runs
+// of seconds by the 1000 W power cap (250 us at 1.70 GHz).
 #include <algorithm>
 
 #include "decode_tile.cuh"
@@ -710,7 +717,7 @@ extern "C" int ecc_decode_paged(const void *q_f16, const void *k_blocks, const v
     }
     if (rc != ECC_OK) return rc;
     // partials per row when the rows are alike; a CTA of one group joins a few of them as fast and three times as
-    // many such CTAs fit an SM (B32 Hq32, 8 partials a row: MERGE_A us against MERGE_B)
+    // many such CTAs fit an SM (B32 Hq32, 7 slots a row: 8.5 us against 14)
     const bool wide = l.slots / ((int64_t)B * Hkv) > 8;
     const cudaError_t e =
         wide ? launch_pdl(paged_merge_kernel<4>, dim3((unsigned)(B * Hq)), dim3(kD * 4), 0, s, a,

@@ -24,6 +24,12 @@
 // r = z - n ln 2 / 512, |r| <= 6.8e-4,
 //   exp(z) = 2^(n div 512) * 2^((n mod 512) / 512) * (1 + r + r^2/2 + r^3/6)
 // (Tang, Table-driven implementation of the exponential function, 1989).
+//
+// Measured per call at 128256 bf16 logits: top-k 50 + top-p 0.9 21 us for one
+// row and 33 us for 64; top-p 0.9 alone 37 and 72 us; no filter 12 and 28 us;
+// greedy 4 and 7 us.  A row alone is bound by the latency of its phases (about
+// a microsecond per cluster barrier with the sums around it); 64 rows by the
+// fp64 exponentials, 0.5 clocks per SM and token.
 #include <cuda_bf16.h>
 
 #include <algorithm>
