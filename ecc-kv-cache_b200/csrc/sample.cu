@@ -71,6 +71,14 @@ template <>
 __device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
 template <>
 __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 // A value's key (cluster_select.cuh).  fp16 values have 10 bits of mantissa
 // behind fp32's exponent, bf16 values 7: the bits below `key_low` say nothing
@@ -115,8 +123,7 @@ struct Mass {
     const double *tab;
     double best, inv_t;
     int S;
-    __device__ __forceinline__ uint64_t operator()(float x) const {
-        if (x == (float)best) return 1ull << S;
+    __device__ __forceinline__ uint64_t operator()(float x) const {  // the maximum itself: exactly 2^S
         const double d = (double)x - best;
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
         const double t = fma(d, inv_t * (kTab / 0.693147180559945309417), kMagic);
@@ -241,8 +248,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 
     const int base = min(a.V, rank * a.slice), n = min(a.V, base + a.slice) - base;
     const T *x_g = reinterpret_cast<const T *>(a.logits) + (int64_t)row * a.row_stride + base;
-    auto load = [x_s, x_g](int i) {
-        const float x = to_float<T>(kCached ? x_s[i] : x_g[i]);
+    // Element i: NaN counts as -inf; with an infinite maximum, the maximum as 0 and all else as -inf (`infinite`).
+    // A slice in shared memory is put that way once.
+    bool infinite = false;
+    auto load = [x_s, x_g, &infinite](int i) {
+        if (kCached) return to_float<T>(x_s[i]);
+        const float x = to_float<T>(x_g[i]);
+        if (infinite) return x == INFINITY ? 0.0f : -INFINITY;
         return x != x ? -INFINITY : x;
     };
 
@@ -261,7 +273,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 #pragma unroll 4
     for (int i = tid; i < n; i += kThreads) {
         const float x = load(i);
-        if (x > best) best = x, best_at = base + i;  // ascending i: the first of equals
+        if (kCached && x != x) x_s[i] = from_float<T>(-INFINITY);
+        if (x > best) best = x, best_at = base + i;  // ascending i: the first of equals; not a NaN
     }
     auto better = [](float x, uint32_t i, float &bx, uint32_t &bi) {
         if (x > bx || (x == bx && i < bi)) bx = x, bi = i;
@@ -297,6 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         }
         return;
     }
+    if (best == INFINITY) {  // cluster-uniform
+        if (kCached) {
+            for (int i = tid; i < n; i += kThreads) {  // each thread the elements that it alone has read so far
+                const bool top = to_float<T>(x_s[i]) == INFINITY;
+                x_s[i] = from_float<T>(top ? 0.0f : -INFINITY);
+            }
+        }
+        infinite = true;
+        best = 0.0f;
+    }
+    if (kCached) __syncthreads();  // the slice as the other threads read it from here on
     const Mass mass{wk.tab, (double)best, 1.0 / (double)temp, a.S};
 
     // What is kept so far: keys above `kth`, equal ones below the row position `cut`.
@@ -330,10 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         // x, and spread however the logits lie
         Bins &bins = *reinterpret_cast<Bins *>(sh.hist);
         unsigned long long *list = reinterpret_cast<unsigned long long *>(sh.hist);
-        const float inv_bin = 64.0f / temp;
-        auto distance = [best, inv_bin](float x) {  // in bins; not of the infinite maximum itself
-            return x == best ? 0.0f : (best - x) * inv_bin;
-        };
+        const float inv_bin = fminf(64.0f / temp, 3e38f);
+        auto distance = [best, inv_bin](float x) { return (best - x) * inv_bin; };  // in bins; -inf: infinity or NaN
         auto bin_of = [distance](float x) {
             const float d = distance(x);
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;
@@ -364,8 +386,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                     atomicAdd(&bins.count[b], 1u);
                     if (kMass) atomicAdd(&bins.mass[b], (unsigned long long)w);
                     // the low half of the bin's 64 bits: at most 2^20 tokens, fewer than 2^10 places each
-                    if (kPlaced)
-                        atomicAdd(reinterpret_cast<uint32_t *>(&bins.mass[b]), (uint32_t)((d - (float)b) * kPlaces));
+                    if (kPlaced) {
+                        const float fb = __int_as_float(0x4b000000 | b) - 8388608.0f;  // (float)b
+                        atomicAdd(reinterpret_cast<uint32_t *>(&bins.mass[b]), (uint32_t)((d - fb) * kPlaces));
+                    }
                 }
             }
             far_count = __reduce_add_sync(0xffffffffu, far_count);
@@ -522,34 +546,41 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
                 int lo, hi;
                 warp_part(n, lo, hi);
-                uint64_t all = 0, above = 0, part = 0;
+                uint64_t rest = 0, above = 0, part = 0;
                 constexpr int kTake = 4;
-                for (int i0 = lo; i0 < hi; i0 += 32 * kTake) {
-                    bool hit[kTake], any = false;
+                auto add_up = [&](auto by_min) {  // with min-p the kept masses are not all of those above
+                    for (int i0 = lo; i0 < hi; i0 += 32 * kTake) {
+                        bool hit[kTake], any = false;
 #pragma unroll
-                    for (int q = 0; q < kTake; ++q) {
-                        const int i = i0 + 32 * q + lane;
-                        hit[q] = false;
-                        if (i < hi) {
-                            const float x = load(i), d = distance(x);
+                        for (int q = 0; q < kTake; ++q) {
+                            const int i = i0 + 32 * q + lane;
+                            const float x = i < hi ? load(i) : -INFINITY, d = distance(x);
                             const uint64_t w = mass(x);
-                            const bool in = d < d0;
-                            all += w;
-                            above += in ? w : 0;
-                            part += in && w >= least ? w : 0;
-                            hit[q] = !in && !(d >= d1);
+                            if (d < d0) {
+                                above += w;
+                                if (decltype(by_min)::value) part += w >= least ? w : 0;
+                            } else {
+                                rest += w;
+                            }
+                            hit[q] = i < hi && !(d < d0) && !(d >= d1);
                             any = any || hit[q];
                         }
-                    }
-                    if (!__any_sync(0xffffffffu, any)) continue;
+                        if (!__any_sync(0xffffffffu, any)) continue;
 #pragma unroll
-                    for (int q = 0; q < kTake; ++q) append(hit[q], i0 + 32 * q + lane);
+                        for (int q = 0; q < kTake; ++q) append(hit[q], i0 + 32 * q + lane);
+                    }
+                };
+                if (least > 0) {
+                    add_up(std::true_type());
+                } else {
+                    add_up(std::false_type());
+                    part = above;
                 }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
                 if (lane == 0) wk.part[warp] = part;
-                const ulonglong2 sums = cluster_sum2(sh, cl, all, above);
-                const uint64_t want = want_of(sums.x);
+                const ulonglong2 sums = cluster_sum2(sh, cl, rest, above);
+                const uint64_t want = want_of(sums.x + sums.y);
                 above = sums.y;
                 const int m = sorted();
                 if (rank == 0) {
