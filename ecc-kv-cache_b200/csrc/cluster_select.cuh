@@ -265,17 +265,46 @@ static inline int cluster_size(int64_t rows, int64_t n, int sms, int most, int l
 // Entries of a list of 64-bit words in the place of a pass's bins.
 constexpr int kList = sizeof(Shared::hist) / 8;
 
-// Descending sort of the first power of two >= n entries (those from n on must
-// be zero) of `x` by the whole block.
+// Descending bitonic sort of the first n entries of `x` by the whole block; the
+// entries from n up to the next power of two (at least 32) are overwritten.  Up
+// to 1024 entries a thread holds one: partners within a warp are exchanged by
+// shuffles, only strides of 32 and more go through shared memory, and only the
+// warps that hold entries meet at those barriers (64 entries: 0.5 us, where a
+// block barrier per stride took 3).
 __device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
-    int size = 1;
+    int size = 32;
     while (size < n) size *= 2;
+    const int t = threadIdx.x;
+    if (size <= kThreads) {
+        if (t < size) {
+            unsigned long long v = t < n ? x[t] : 0ull;
+            for (int k = 2; k <= size; k *= 2)
+                for (int j = k / 2; j > 0; j /= 2) {
+                    unsigned long long u;
+                    if (j < 32) {
+                        u = __shfl_xor_sync(0xffffffffu, v, j);
+                    } else {
+                        asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");  // earlier readers are done
+                        x[t] = v;
+                        asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");
+                        u = x[t ^ j];
+                    }
+                    v = (((t & j) == 0) == ((t & k) == 0)) == (v < u) ? u : v;
+                }
+            asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");
+            x[t] = v;
+        }
+        __syncthreads();
+        return;
+    }
+    for (int i = n + t; i < size; i += kThreads) x[i] = 0;
+    __syncthreads();
     for (int k = 2; k <= size; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += kThreads) {
-                const int i = 2 * t - (t & (j - 1));  // bit j of i is clear
-                const unsigned long long p = x[i], q = x[i + j];
-                if ((p < q) == ((i & k) == 0)) x[i] = q, x[i + j] = p;
+            for (int p = t; p < size / 2; p += kThreads) {
+                const int i = 2 * p - (p & (j - 1));  // bit j of i is clear
+                const unsigned long long a = x[i], b = x[i + j];
+                if ((a < b) == ((i & k) == 0)) x[i] = b, x[i + j] = a;
             }
             __syncthreads();
         }

@@ -159,10 +159,6 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
         cl.sync();
         if (rank == 0) {
             const int m = (int)sh.listed;
-            int size = 1;
-            while (size < m) size *= 2;
-            for (int i = m + tid; i < size; i += sel::kThreads) list[i] = 0;
-            __syncthreads();
             sel::sort_descending(list, m);
             if (tid < C) {
                 const unsigned long long e = list[k - (int)at_k.before - 1];

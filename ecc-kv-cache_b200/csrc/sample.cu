@@ -421,13 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         auto sorted = [&]() {
             cl.sync();
             const int m = min((int)wk.listed, kList);
-            if (rank == 0) {
-                int size = 1;
-                while (size < m) size *= 2;
-                for (int i = m + tid; i < size; i += kThreads) list[i] = 0;
-                __syncthreads();
-                sort_descending(list, m);
-            }
+            if (rank == 0) sort_descending(list, m);
             return m;
         };
         // The kept tokens of bins b0 .. b1 in the list, sorted.
@@ -496,9 +490,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 }
                 // by row position, and the draw
                 for (int i = tid; i < kept; i += kThreads) list[i] = (list[i] << 32) | (list[i] >> 32);
-                int size = 1;
-                while (size < kept) size *= 2;
-                for (int i = kept + tid; i < size; i += kThreads) list[i] = 0;
                 __syncthreads();
                 sort_descending(list, kept);
                 auto drawn_mass = [&](int i) { return mass(key_value<T>((uint32_t)list[i])); };
