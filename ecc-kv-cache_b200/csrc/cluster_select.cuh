@@ -151,7 +151,9 @@ __device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_gro
         }
     }
     cl.sync();
-    return cs.found;
+    Crossing f = cs.found;
+    f.slot &= kBins - 1;  // a bin in any case
+    return f;
 }
 
 // The k-th largest key of the cluster's row, 1 <= k <= keys of the row.

@@ -184,6 +184,12 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     const int64_t tbeg = wid * T / NW;
     const int ntiles = (int)((wid + 1) * T / NW - tbeg);
 
+    // a sequence's tiles; their number is the one that the cut was made with
+    auto tiles_of = [&](int b) {
+        SeqTiles st(seq_len_of(a, b), a.window, a.sinks);
+        st.n = s_pre[b + 1] - s_pre[b];
+        return st;
+    };
     Cursor cons;
     {
         int lo = 0, hi = a.B - 1;  // last sequence whose first tile is <= tbeg
@@ -193,7 +199,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             else hi = mid - 1;
         }
         cons.b = lo;
-        cons.st = SeqTiles(seq_len_of(a, lo), a.window, a.sinks);
+        cons.st = tiles_of(lo);
         const int rest = (int)(tbeg - (int64_t)s_pre[lo] * Hkv);
         cons.h = rest / cons.st.n;
         cons.u = rest - cons.h * cons.st.n;
@@ -205,7 +211,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             k.h = 0;
             do ++k.b;
             while (k.b < a.B && s_pre[k.b + 1] == s_pre[k.b]);
-            if (k.b < a.B) k.st = SeqTiles(seq_len_of(a, k.b), a.window, a.sinks);
+            if (k.b < a.B) k.st = tiles_of(k.b);
         }
     };
 

@@ -87,7 +87,11 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
         return;
     }
     const int b = row / a.Hkv, h = row - b * a.Hkv;
-    int L = __ldg(a.lens + b);
+    // one thread reads the length for the whole cluster, which branches on it together
+    if (tid == 0) sh.listed = (uint32_t)__ldg(a.lens + b);
+    cl.sync();
+    int L = (int)*sel::of_rank(cl, &sh.listed, 0);
+    cl.sync();
     if (L < 0 || L > a.src.capacity) {
         if (tid == 0 && rank == 0) atomicExch(&g_paged_error, 5);
         L = max(0, min(L, a.src.capacity));
@@ -154,14 +158,14 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
             uint32_t at = 0;
             if (lane == 0) at = atomicAdd(sel::of_rank(cl, &sh.listed, 0), (uint32_t)__popc(m));
             at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
-            if (hit) sel::of_rank(cl, list, 0)[at] = ((unsigned long long)x << 32) | (uint32_t)~(uint32_t)(base + i0 + lane);
+            if (hit && at < sel::kList) sel::of_rank(cl, list, 0)[at] = ((unsigned long long)x << 32) | (uint32_t)~(uint32_t)(base + i0 + lane);
         }
         cl.sync();
         if (rank == 0) {
-            const int m = (int)sh.listed;
+            const int m = min((int)sh.listed, sel::kList);
             sel::sort_descending(list, m);
             if (tid < C) {
-                const unsigned long long e = list[k - (int)at_k.before - 1];
+                const unsigned long long e = list[(k - (int)at_k.before - 1) & (sel::kList - 1)];
                 *sel::of_rank(cl, &sh.cta_b, tid) = (uint32_t)(e >> 32);
                 *sel::of_rank(cl, &sh.cut, tid) = ~(uint32_t)e + 1;
             }
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
         const uint32_t m = __ballot_sync(0xffffffffu, hit);
         const int to = (int)(at + __popc(m & ((1u << lane) - 1u))), t = base + i0 + lane;
         // the weight again out of its key (-0 comes back as +0)
-        if (hit) put_as(to, t, cached ? key_weight(cache[i0 + lane]) : __ldg(w + t));
+        if (hit && to < a.budget - a.recent) put_as(to, t, cached ? key_weight(cache[i0 + lane]) : __ldg(w + t));
         at += __popc(m);
     }
 }

@@ -43,7 +43,7 @@ struct PageTable {
     __device__ __forceinline__ int page(int b, int t, int &slot) const {
         const uint32_t pi = page_of(t);
         slot = t - (int)pi * page_size;
-        const int p = __ldg(table + b * stride + pi);
+        const int p = pi < (uint32_t)width ? __ldg(table + b * stride + pi) : -1;
         if ((uint32_t)p < (uint32_t)n_pages) return p;
         atomicExch(&g_paged_error, 5);
         return -1;

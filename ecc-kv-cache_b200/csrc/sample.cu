@@ -94,8 +94,13 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~(k | ~(0xffffffffu << key_low<T>())));
 }
 
+struct Settings {  // of a row
+    float temp, top_p, min_p, u;
+    int top_k;
+};
 struct Work {
     Shared sel;
+    Settings first, set;  // as this CTA read them; the cluster's: the first CTA's
     unsigned long long tot_mass[kBins];  // the cluster's masses and counts, this CTA's share of the bins
     uint32_t tot_count[kBins];
     double tab[kTab];
@@ -245,6 +250,14 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     if (tid == 0) wk.listed = 0;
     pdl_trigger();
     pdl_wait();
+    // one thread reads the row's settings for the whole cluster, which branches on them together
+    if (tid == 0) {
+        wk.first.temp = a.temperature ? __ldg(a.temperature + row) : a.temperature0;
+        wk.first.top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p0;
+        wk.first.min_p = a.min_p ? __ldg(a.min_p + row) : a.min_p0;
+        wk.first.u = __ldg(a.u + row);
+        wk.first.top_k = a.top_k ? __ldg(a.top_k + row) : a.top_k0;
+    }
 
     const int base = min(a.V, rank * a.slice), n = min(a.V, base + a.slice) - base;
     const T *x_g = reinterpret_cast<const T *>(a.logits) + (int64_t)row * a.row_stride + base;
@@ -297,12 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         best = -INFINITY, best_at = 0xffffffffu;
         if (lane < C) best = *of_rank(cl, &wk.cta_best, lane), best_at = *of_rank(cl, &wk.cta_best_at, lane);
         warp_best();
-        if (lane == 0) wk.best = best, wk.best_at = best_at;
+        if (lane == 0) wk.best = best, wk.best_at = best_at, wk.set = *of_rank(cl, &wk.first, 0);
     }
     cl.sync();  // also: nobody reads a CTA's shared memory after it may have left
     best = wk.best;
     best_at = wk.best_at;
-    const float temp = a.temperature ? __ldg(a.temperature + row) : a.temperature0;
+    const float temp = wk.set.temp;
     if (best == -INFINITY || !(temp > 0.0f)) {  // cluster-uniform
         if (rank == 0 && tid == 0) {
             a.token[row] = best == -INFINITY ? -1 : (int64_t)best_at;
@@ -328,13 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     auto key = [&](int i) { return value_key<T>(load(i)); };
     auto keep = [&](uint32_t x, int i) { return x > kth || (x == kth && (uint32_t)(base + i) < cut); };
 
-    const int k = a.top_k ? __ldg(a.top_k + row) : a.top_k0;
-    const float p = a.top_p ? __ldg(a.top_p + row) : a.top_p0;
+    const int k = wk.set.top_k;
+    const float p = wk.set.top_p;
     const bool by_count = k > 0 && k < a.V, by_mass = p < 1.0f;
-    const float mp = a.min_p ? __ldg(a.min_p + row) : a.min_p0;
+    const float mp = wk.set.min_p;
     // w >= min_p as whole masses; the most likely token stays in any case
     const uint64_t least = mp > 0.0f ? (uint64_t)ceil(fmin((double)mp, 1.0) * (double)(1ull << a.S)) : 0;
-    const float u = __ldg(a.u + row);
+    const float u = wk.set.u;
     // cumulative mass > u * total, of whole masses: > floor(u * total); a number of 1 or more takes the last
     // kept token, one that is not above 0 the first
     auto need_of = [u](uint64_t total) -> uint64_t {
@@ -608,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             if (at_k.here <= kList) {
                 const int m = gather(b, b);
                 if (rank == 0) {
-                    if (tid == 0) publish(list[rest - 1]);
+                    if (tid == 0) publish(list[(rest - 1) & (kList - 1)]);
                     uint64_t mine = 0;
                     if (by_mass)
                         for (int i = rest + tid; i < m; i += kThreads) mine += listed_mass(i);

@@ -93,6 +93,22 @@ def test_evict_equal_and_special_weights(weights, budget):
     check([700, 250], 2, 16, 128, budget, 2, 9, weights=weights, seed=budget)
 
 
+def _one_value(rng, B, H, n):
+    return np.full((B, H, n), 0.125)
+
+
+def _three_values(rng, B, H, n):
+    w = rng.integers(0, 3, (B, H, n)) * 0.25
+    w[..., ::7] = rng.random((B, H, w[..., ::7].shape[-1]))
+    return w
+
+
+@pytest.mark.parametrize("weights", [_one_value, _three_values])
+@pytest.mark.parametrize("B,hkv", [(1, 1), (20, 3)])  # one row by a cluster, one CTA per row
+def test_evict_more_equal_weights_than_the_list_holds(weights, B, hkv):
+    check([20011 - 100 * b for b in range(B)], hkv, 64, 96, 9000, 4, 100, weights=weights, seed=B, spare=1)
+
+
 def test_evict_one_long_row():
     check([20011], 1, 16, 128, 9000, 4, 100, seed=1)
 

@@ -109,6 +109,20 @@ def test_sample_equal_logits(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_sample_more_equal_logits_than_the_list_holds(dtype):
+    u = torch.tensor([0.0, 0.1, 0.25, 0.4999999, 0.5, 0.75, 0.999999], device="cuda")
+    x = torch.full((7, 30000), -1.5, dtype=TYPES[dtype], device="cuda")
+    for s in (dict(), dict(k=10), dict(k=20000), dict(p=0.5), dict(k=20000, p=0.25), dict(mp=1.0), dict(T=0.0)):
+        check(x, u, **s)
+    x[:, ::3] = 0.75  # 10000 and 20000 of two values, and a few others
+    x[:, 5::1001] = -0.0
+    x[:, 7::999] = 3.0
+    for s in (dict(), dict(k=10), dict(k=9000), dict(k=25000), dict(p=0.5), dict(p=0.97), dict(k=25000, p=0.99),
+              dict(k=9000, p=0.999), dict(T=0.3, p=0.9999), dict(k=20000, p=0.6, mp=0.01)):
+        check(x, u, **s)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_sample_masks_infinities_and_nan(dtype):
     x, u = rows(8, 700, dtype, seed=3)
     inf = float("inf")
