@@ -11,6 +11,8 @@
 #pragma once
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "ecc_common.cuh"
 
 namespace ecc {
@@ -256,11 +258,42 @@ __device__ __forceinline__ uint32_t tie_cut(Shared &sh, cg::cluster_group &cl, i
     return cut;
 }
 
-// Cluster size for `rows` rows of `n` elements: the largest power of two up to
-// `most` with which every CTA still has an SM of its own and `least` elements.
-static inline int cluster_size(int64_t rows, int64_t n, int sms, int most, int least) {
+// Cluster size for `clusters` clusters that share a row of `n` elements each: the
+// largest power of two up to 8 with which all of them run at the same time and
+// every CTA has `least` elements.  A cluster lives inside one GPC, so fewer fit
+// than the SMs would hold (16 rows in clusters of 8: 21 us in two waves where
+// clusters of 4 take 14).  Asked once per device.
+constexpr size_t kMostShared = 227 * 1024;
+template <typename... KArgs>
+static inline int cluster_size(void (*kernel)(KArgs...), int64_t clusters, int64_t n, int least) {
+    static std::atomic<int> fit[64][4];  // by device and log2 of the size: clusters at a time, plus 1
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
     int c = 1;
-    while (c < most && rows * (2 * c) <= sms && n >= (int64_t)least * 2 * c) c *= 2;
+    for (int lg = 1; lg < 4 && n >= (int64_t)least << lg; ++lg) {
+        int v = fit[dev][lg].load(std::memory_order_relaxed);
+        if (v == 0) {
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(1u << lg);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = kMostShared;  // one CTA per SM
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim = {1u << lg, 1, 1};
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int most = 0;
+            if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                most = 0;
+            }
+            v = most + 1;
+            fit[dev][lg].store(v, std::memory_order_relaxed);
+        }
+        if (clusters > v - 1) break;
+        c = 1 << lg;
+    }
     return c;
 }
 
@@ -317,7 +350,7 @@ __device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_cluster(void (*kernel)(KArgs...), int c, int64_t rows, size_t smem, cudaStream_t s,
                                          Args &&...args) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(c * rows));

@@ -311,7 +311,7 @@ extern "C" int ecc_evict_paged(void *k_blocks, void *v_blocks, int64_t bs_p, int
 
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const int64_t rows = (int64_t)B * Hkv;
-    const int C = sel::cluster_size(rows, a.src.capacity, sm_count(), 8, 4096);
+    const int C = sel::cluster_size(evict_select_kernel, rows + 1, a.src.capacity, 4096);
     // the keys of a slice stay in shared memory when they fit beside the counts
     const int64_t slice = (a.src.capacity + C - 1) / C;
     a.cache_keys = (int)std::min<int64_t>(slice, (227 * 1024 - sizeof(sel::Shared)) / 4);

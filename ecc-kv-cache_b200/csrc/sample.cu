@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 template <class T>
 static int launch(Args &a, cudaStream_t s) {
     constexpr size_t kHead = (sizeof(Work) + 15) / 16 * 16, kRoom = 227 * 1024 - kHead;
-    int C = cluster_size(a.B, a.V, sm_count(), 8, 2048);
+    int C = cluster_size(sample_kernel<T, true>, a.B, a.V, 2048);
     while (C < 8 && (size_t)(a.V + C - 1) / C * sizeof(T) > kRoom - 64) C *= 2;
     a.slice = ((a.V + C - 1) / C + 15) / 16 * 16;  // slices start 16-byte aligned when the row does
     const size_t bytes = (size_t)a.slice * sizeof(T);
