@@ -226,6 +226,10 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
             if (i >= total) continue;
             const int t = __ldg(a.e.kept + i);
             if (t < 0) continue;
+            if (t >= a.e.src.capacity) {  // the caller wrote to `kept` during the call
+                atomicExch(&g_paged_error, 5);
+                continue;
+            }
             const uint32_t row = fdiv(i, div_n), b = fdiv(row, div_h);
             const int h = (int)(row - b * div_h.d), o = (int)(i - row * div_n.d);
             int ss, ds;

@@ -39,11 +39,11 @@ struct PageTable {
     int capacity;  // tokens a row of the table can name
     FastDiv div;
     __device__ __forceinline__ uint32_t page_of(int t) const { return fdiv((uint32_t)t, div); }
-    // page of token t of sequence b, or -1 (flagged) when the table names none
+    // page of token t < capacity of sequence b, or -1 (flagged) when the table names none
     __device__ __forceinline__ int page(int b, int t, int &slot) const {
         const uint32_t pi = page_of(t);
         slot = t - (int)pi * page_size;
-        const int p = pi < (uint32_t)width ? __ldg(table + b * stride + pi) : -1;
+        const int p = __ldg(table + b * stride + pi);
         if ((uint32_t)p < (uint32_t)n_pages) return p;
         atomicExch(&g_paged_error, 5);
         return -1;

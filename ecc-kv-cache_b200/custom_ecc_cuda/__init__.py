@@ -967,11 +967,6 @@ def _weights_like(t: torch.Tensor, name: str, B: int, hkv: int, capacity: int, d
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
-def _span(t: torch.Tensor) -> int:
-    """Bytes from a tensor's first element to its last."""
-    return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else 0
-
-
 def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
                         block_table: torch.Tensor, pos: torch.Tensor, new_lens: torch.Tensor | None = None,
                         rotate: bool = True) -> None:
@@ -1099,6 +1094,11 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     return (out, lse) if return_lse else out
 
 
+@functools.lru_cache(1024)
+def _evict_paged_bytes(n_pages: int) -> int:
+    return int(_lib.ecc_evict_paged_workspace_size(n_pages))
+
+
 def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                 weights: torch.Tensor, out_table: torch.Tensor, budget: int, sinks: int = 0, recent: int = 0,
                 out_weights: torch.Tensor | None = None, kept: torch.Tensor | None = None,
@@ -1135,15 +1135,20 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out_weights is None:
         out_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
-    op, ob, oh = _weights_like(out_weights, "out_weights", B, hkv, capacity, dev)
-    if op < wp + _span(weights) and wp < op + _span(out_weights):
-        raise RuntimeError("out_weights must not share memory with weights")
+        op, (ob, oh, _) = out_weights.data_ptr(), out_weights.stride()
+    else:
+        op, ob, oh = _weights_like(out_weights, "out_weights", B, hkv, capacity, dev)
+        # from the first element to the last, in bytes
+        span, out_span = (4 * ((B - 1) * sb + (hkv - 1) * sh + t.shape[2]) if B else 0
+                          for t, sb, sh in ((weights, wb, wh), (out_weights, ob, oh)))
+        if op < wp + span and wp < op + out_span:
+            raise RuntimeError("out_weights must not share memory with weights")
     if kept is None:
         kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
     elif tuple(kept.shape) != (B, hkv, budget) or kept.dtype is not torch.int32 or not kept.is_contiguous() \
             or kept.device != dev:
         raise RuntimeError("kept must be a contiguous int32 tensor [B, Hkv, budget] on the pools' device")
-    ws = _scratch(workspace, dev, _lib.ecc_evict_paged_workspace_size(shape[0]))
+    ws = _scratch(workspace, dev, _evict_paged_bytes(shape[0]))
     _launch(_lib.ecc_evict_paged, "evict_paged", dev, k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1], pages, lens,
             wp, wb, wh, outs, op, ob, oh, out_weights.shape[2], kept.data_ptr(), B, hkv, int(budget), int(sinks),
             int(recent), shape[3], ws.data_ptr(), ws.numel() * ws.element_size())
