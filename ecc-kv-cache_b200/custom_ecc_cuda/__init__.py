@@ -881,13 +881,19 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 # ---------------------------------------------------------------------------
 # Paged cache: sequences of any lengths in pages of a shared pool
 # ---------------------------------------------------------------------------
+_launch_locks = tuple(threading.Lock() for _ in range(64))  # by device
+
+
 def _launch(fn, what: str, dev: torch.device, *args) -> None:
-    """fn(*args, current stream of dev) with dev the current device."""
+    """fn(*args, current stream of dev) with dev the current device.  One call
+    at a time: the launches of a call share a workspace, and those of another
+    thread on the same stream must not come between them."""
     i = dev.index
     if torch.cuda.current_device() == i:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+        with _launch_locks[i & 63]:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(dev), _launch_locks[i & 63]:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         _check(rc, what)
@@ -959,12 +965,17 @@ def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> int:
     return t.data_ptr()
 
 
-def _weights_like(t: torch.Tensor, name: str, B: int, hkv: int, capacity: int, dev) -> tuple:
+def _weights_like(t: torch.Tensor, name: str, B: int, hkv: int, capacity: int, dev, written: bool = True) -> tuple:
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.dim() != 3 or t.device != dev \
             or t.shape[0] != B or t.shape[1] != hkv or t.shape[2] < capacity or t.stride(2) != 1:
         raise RuntimeError(f"{name} must be float32 [B, Hkv, >= {capacity}] with a contiguous last dimension on the "
                            f"pools' device")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    sb, sh = t.stride(0), t.stride(1)
+    if written:  # the rows of all sequences and heads lie apart
+        (near, n), (far, m) = ((sh, hkv), (sb, B)) if B < 2 or (hkv > 1 and sh <= sb) else ((sb, B), (sh, hkv))
+        if (n > 1 and near < t.shape[2]) or (m > 1 and far < (near * (n - 1) if n > 1 else 0) + t.shape[2]):
+            raise RuntimeError(f"{name} must not hold the same element twice (its rows overlap)")
+    return t.data_ptr(), sb, sh
 
 
 def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.Tensor, v_pool: torch.Tensor | None,
@@ -1132,7 +1143,7 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     if outs.table == pages.table:
         raise RuntimeError("out_table must name other pages than block_table")
     capacity = pages.width * pages.page_size
-    wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev)
+    wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev, written=False)
     if out_weights is None:
         out_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
         op, (ob, oh, _) = out_weights.data_ptr(), out_weights.stride()

@@ -51,6 +51,8 @@ class GraphDecoder:
         self.cache_position = torch.full((1,), self.n0, dtype=torch.long, device=dev)
         self.position_ids = torch.full((B, 1), self.n0, dtype=torch.long, device=dev)
         self.sampler = sampler
+        # the recorded draw reads these tensors, whatever the sampler is given later
+        self._settings = None if sampler is None else (sampler.temperature, sampler.top_k, sampler.top_p, sampler.min_p)
         self.uniform = torch.zeros(B, dtype=torch.float32, device=dev)  # the numbers of the next draw
         fills = list(cache._layer_fill)
         # one eager step off the capture: workspaces, tensor maps, kernel

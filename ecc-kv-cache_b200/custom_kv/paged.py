@@ -162,6 +162,8 @@ class PagedErrorCorrectedCache(_HFCache):
         if d != HEAD_DIM or H != self.num_heads or B != self.batch_size:
             raise RuntimeError(f"append: expected [B={self.batch_size}, H={self.num_heads}, L, 128], "
                                f"got {tuple(key_states.shape)}")
+        if value_states.shape != key_states.shape:
+            raise RuntimeError(f"append: keys {tuple(key_states.shape)} and values {tuple(value_states.shape)} differ")
         new = [L] * B if new_lens is None else [int(n) for n in new_lens]
         if len(new) != B or min(new) < 0 or max(new) > L:
             raise RuntimeError(f"new_lens must hold {B} counts from 0 to {L}")

@@ -232,6 +232,33 @@ def test_decode_on_a_side_stream():
     assert all(torch.equal(o, ref) for o in outs)
 
 
+def test_decode_from_two_threads_on_one_stream():
+    import threading
+    import custom_ecc_cuda as ops
+    rng = np.random.default_rng(16)
+    cases = []
+    for lens, hkv in (([4000, 17, 900], 2), ([2500, 3100], 4)):
+        kp, vp, table = R.make_pools(lens, 64, hkv, 128, rng)
+        q = cu(rng.normal(size=(len(lens), 4 * hkv, 128)).astype(np.float16))
+        args = (q, cu(kp), cu(vp), cu(table), i32(lens))
+        cases.append((args, ops.decode_attention_paged(*args)))
+    torch.cuda.synchronize()
+    outs = [[], []]
+
+    def run(i):
+        for _ in range(200):
+            outs[i].append(ops.decode_attention_paged(*cases[i][0]))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(outs[i]) == 200 and all(torch.equal(o, cases[i][1]) for o in outs[i])
+
+
 # ------------------------------------------------------------------ append and read-back
 @pytest.mark.parametrize("L,hkv,ps,rec", [(1, 2, 16, 128), (17, 3, 32, 96), (40, 1, 48, 128), (700, 4, 64, 128),
                                           (700, 4, 64, 96)])

@@ -190,6 +190,26 @@ def test_model_runs_on_the_paged_cache(cuda_device):
             assert float(cache.weights.sum()) <= 6 * 2 * 2 * 4 * (1 + 1e-4)
 
 
+def test_recorded_settings_outlive_the_sampler(cuda_device):
+    import custom_ecc_cuda as ops
+    from custom_kv import Sampler, ecc_cache
+    from custom_kv.graph import GraphDecoder
+    model = _tiny_llama(3)
+    ids = torch.randint(0, 1000, (2, 40), generator=torch.Generator().manual_seed(4)).cuda()
+    with torch.no_grad(), ecc_cache(model, batch_size=2, max_cache_len=128) as cache:
+        logits = model(ids, past_key_values=cache, use_cache=True).logits[:, -1]
+        sampler = Sampler(temperature=torch.tensor([0.9, 0.5], device="cuda"))
+        dec = GraphDecoder(model, cache, sampler(logits)[:, None], sampler=sampler)
+        sampler.temperature = 1.0  # the record goes on with the tensor that it was made with
+        torch.cuda.empty_cache()
+        taken = [torch.full((2,), 7.0, device="cuda") for _ in range(64)]
+        for u in ([0.1, 0.9], [0.7, 0.3]):
+            u = torch.tensor(u, device="cuda")
+            t = dec.step(u)
+            assert torch.equal(t[:, 0], ops.sample_tokens(dec.logits, u, temperature=torch.tensor([0.9, 0.5], device="cuda")))
+        assert len(taken) == 64
+
+
 def test_graph_decoder_samples(cuda_device):
     import custom_ecc_cuda as ops
     from custom_kv import Sampler, ecc_cache

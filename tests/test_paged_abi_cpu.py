@@ -159,3 +159,22 @@ def test_paged_cache_refuses_cpu_device():
     cfg = types.SimpleNamespace(num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=2, hidden_size=256)
     with pytest.raises(RuntimeError, match="CUDA"):
         PagedErrorCorrectedCache(cfg, device="cpu")
+
+
+def test_written_weights_must_not_overlap():
+    import custom_ecc_cuda as ops
+    cpu = torch.device("cpu")
+
+    def look(t, B, H, **kw):
+        return ops._weights_like(t, "weights", B, H, 32, cpu, **kw)
+
+    whole = torch.zeros(3, 2, 40)
+    for t in (whole, whole[:, :, 4:], whole[:2], whole.transpose(0, 1).contiguous().transpose(0, 1), whole[:, :1], whole[:1],
+              torch.zeros(6, 2, 40)[::2], torch.zeros(1, 1, 32).expand(1, 1, 32)):
+        assert look(t, t.shape[0], t.shape[1]) == (t.data_ptr(), t.stride(0), t.stride(1))
+    for t in (torch.zeros(1, 2, 40).expand(3, 2, 40), torch.zeros(3, 1, 40).expand(3, 2, 40),
+              torch.zeros(1, 1, 40).expand(3, 1, 40), torch.zeros(200).as_strided((3, 2, 40), (40, 39, 1)),
+              torch.zeros(300).as_strided((3, 2, 40), (79, 40, 1)), torch.zeros(300).as_strided((3, 2, 40), (40, 119, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            look(t, t.shape[0], t.shape[1])
+        look(t, t.shape[0], t.shape[1], written=False)  # to be read only
