@@ -33,7 +33,7 @@ struct Crossing {  // see crossing()
 };
 struct CrossingShared {
     uint64_t share[kMaxCluster];  // the CTAs' sums of their bins, written by each of them
-    Crossing found;               // written by the CTA that finds it
+    Crossing found[2];            // written by the CTA that finds it
 };
 
 struct alignas(16) Shared {
@@ -91,8 +91,8 @@ __device__ __forceinline__ T block_exclusive(T v, T *warp_sums, T *total) {
 // r W + W), W = kBins / CTAs, in to[0 .. W).  All CTAs must have passed a
 // cluster barrier since their `from` was written, and pass one (crossing()
 // does) before it is written again.
-template <class T>
-__device__ __forceinline__ void cluster_share(cg::cluster_group &cl, T *from, T *to) {
+template <class T, class U>
+__device__ __forceinline__ void cluster_share(cg::cluster_group &cl, T *from, U *to) {
     const int ranks = (int)cl.num_blocks(), W = kBins / ranks, at = (int)cl.block_rank() * W;
     for (int i = threadIdx.x; i < W; i += kThreads) {
         T c = 0;
@@ -124,16 +124,19 @@ __device__ __forceinline__ uint64_t share_sums(CrossingShared &cs, cg::cluster_g
     return all;
 }
 // Where the running sum over the spread bins, whose share_sums() are known,
-// reaches `want` (1 <= want <= the sum of all): the bin, the sum before it and
-// its own, the same in every CTA.  Ends with a cluster barrier.
-template <class T>
-__device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_group &cl, const T *bins, uint64_t want,
-                                             uint64_t *warp_sums) {
+// reaches want[j] (1 <= want[j] <= the sum of all): the bin, the sum before it
+// and its own, the same in every CTA.  Ends with a cluster barrier.
+template <class T, int K>
+__device__ __forceinline__ void crossings(CrossingShared &cs, cg::cluster_group &cl, const T *bins,
+                                          const uint64_t (&want)[K], Crossing (&found)[K], uint64_t *warp_sums) {
     const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), W = kBins / ranks;
     uint64_t before = 0;
     for (int r = 0; r < rank; ++r) before += cs.share[r];
     const uint64_t mine = cs.share[rank];
-    if (before < want && want <= before + mine) {  // block-uniform
+    bool here = false;
+#pragma unroll
+    for (int j = 0; j < K; ++j) here = here || (before < want[j] && want[j] <= before + mine);
+    if (here) {  // block-uniform
         const int per = (W + kThreads - 1) / kThreads;
         uint64_t v[kPerThread], sum = 0;
 #pragma unroll
@@ -146,16 +149,28 @@ __device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_gro
         before += block_exclusive(sum, warp_sums, &all);
 #pragma unroll
         for (int j = 0; j < kPerThread; ++j) {
-            if (before < want && want <= before + v[j])
-                for (int r = 0; r < ranks; ++r)
-                    of_rank(cl, &cs, r)->found = {(uint32_t)(rank * W + threadIdx.x * per + j), before, v[j]};
+#pragma unroll
+            for (int q = 0; q < K; ++q)
+                if (before < want[q] && want[q] <= before + v[j])
+                    for (int r = 0; r < ranks; ++r)
+                        of_rank(cl, &cs, r)->found[q] = {(uint32_t)(rank * W + threadIdx.x * per + j), before, v[j]};
             before += v[j];
         }
     }
     cl.sync();
-    Crossing f = cs.found;
-    f.slot &= kBins - 1;  // a bin in any case
-    return f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+        found[j] = cs.found[j];
+        found[j].slot &= kBins - 1;  // a bin in any case
+    }
+}
+template <class T>
+__device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_group &cl, const T *bins, uint64_t want,
+                                             uint64_t *warp_sums) {
+    const uint64_t w[1] = {want};
+    Crossing f[1];
+    crossings(cs, cl, bins, w, f, warp_sums);
+    return f[0];
 }
 
 // The k-th largest key of the cluster's row, 1 <= k <= keys of the row.
@@ -258,6 +273,28 @@ __device__ __forceinline__ uint32_t tie_cut(Shared &sh, cg::cluster_group &cl, i
     return cut;
 }
 
+// Entries of a list of 64-bit words in the place of a pass's bins.
+constexpr int kList = sizeof(Shared::hist) / 8;
+
+// Moves the entries that every CTA put into its own list (room for kList, their
+// number in *listed) behind one another into the first CTA's.  All CTAs have
+// passed a cluster barrier since their last entry; ends with one.  Returns the
+// number of all entries; nothing is moved when that is more than kList.
+__device__ __forceinline__ uint32_t join_lists(cg::cluster_group &cl, unsigned long long *list, const uint32_t *listed) {
+    const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    uint32_t before = 0, mine = 0, all = 0;
+    for (int r = 0; r < ranks; ++r) {
+        const uint32_t c = *of_rank(cl, const_cast<uint32_t *>(listed), r);
+        if (r < rank) before += c;
+        if (r == rank) mine = c;
+        all += c;
+    }
+    if (rank > 0 && all <= (uint32_t)kList)
+        for (int i = threadIdx.x; i < (int)mine; i += kThreads) of_rank(cl, list, 0)[before + i] = list[i];
+    cl.sync();
+    return all;
+}
+
 // Cluster size for `clusters` clusters that share a row of `n` elements each: the
 // largest power of two up to 8 with which all of them run at the same time and
 // every CTA has `least` elements.  A cluster lives inside one GPC, so fewer fit
@@ -296,9 +333,6 @@ static inline int cluster_size(void (*kernel)(KArgs...), int64_t clusters, int64
     }
     return c;
 }
-
-// Entries of a list of 64-bit words in the place of a pass's bins.
-constexpr int kList = sizeof(Shared::hist) / 8;
 
 // Descending bitonic sort of the first n entries of `x` by the whole block; the
 // entries from n up to the next power of two (at least 32) are overwritten.  Up

@@ -149,21 +149,25 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
     sel::share_sums(sh.cross, cl, sh.tot, sh.warp64);
     const sel::Crossing at_k = sel::crossing(sh.cross, cl, sh.tot, (uint64_t)k, sh.warp64);
     if (at_k.here <= sel::kList) {
+        // few entries go straight to the first CTA, which saves join_lists' barrier
+        const bool at_rank0 = at_k.here <= 512;
         unsigned long long *list = reinterpret_cast<unsigned long long *>(sh.hist);
+        unsigned long long *list_to = at_rank0 ? sel::of_rank(cl, list, 0) : list;
+        uint32_t *listed_to = at_rank0 ? sel::of_rank(cl, &sh.listed, 0) : &sh.listed;
         for (int i0 = tid - lane; i0 < n; i0 += sel::kThreads) {
             const uint32_t x = i0 + lane < n ? key(i0 + lane) : 0;
             const bool hit = i0 + lane < n && bin_of(x) == (int)at_k.slot;
             const uint32_t m = __ballot_sync(0xffffffffu, hit);
             if (!m) continue;
             uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(sel::of_rank(cl, &sh.listed, 0), (uint32_t)__popc(m));
+            if (lane == 0) at = atomicAdd(listed_to, (uint32_t)__popc(m));
             at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
-            if (hit && at < sel::kList) sel::of_rank(cl, list, 0)[at] = ((unsigned long long)x << 32) | (uint32_t)~(uint32_t)(base + i0 + lane);
+            if (hit && at < sel::kList) list_to[at] = ((unsigned long long)x << 32) | (uint32_t)~(uint32_t)(base + i0 + lane);
         }
         cl.sync();
+        const uint32_t all = at_rank0 ? sh.listed : sel::join_lists(cl, list, &sh.listed);
         if (rank == 0) {
-            const int m = min((int)sh.listed, sel::kList);
-            sel::sort_descending(list, m);
+            sel::sort_descending(list, (int)min(all, (uint32_t)sel::kList));
             if (tid < C) {
                 const unsigned long long e = list[(k - (int)at_k.before - 1) & (sel::kList - 1)];
                 *sel::of_rank(cl, &sh.cta_b, tid) = (uint32_t)(e >> 32);

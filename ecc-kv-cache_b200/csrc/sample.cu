@@ -19,17 +19,19 @@
 // ceil(log2 V), at least 42 bits behind the point), so they do not depend on
 // the order of the additions, and atomics give the same bits every time.
 // A drawn token hangs on which side of a sum u * total falls: fp32 exponentials
-// would move one draw in a few thousand, so w is computed in fp64 to 2^-46
-// relative, by table and polynomial: with n = rint(z * 512 / ln 2) and
-// r = z - n ln 2 / 512, |r| <= 6.8e-4,
-//   exp(z) = 2^(n div 512) * 2^((n mod 512) / 512) * (1 + r + r^2/2 + r^3/6)
-// (Tang, Table-driven implementation of the exponential function, 1989).
+// would move one draw in a few thousand, so w is computed in fp64 to 2^-45
+// relative, by table and polynomial:
+//   2^y = 2^n 2^(i / 512) 2^f,  2^f = 1 + c1 f + c2 f^2 + c3 f^3,  ck = ln(2)^k / k!,
+// |f| <= 2^-10: the polynomial is off by 2^-46.7 (Tang, Table-driven implementation
+// of the exponential function, 1989).
 //
-// Measured per call at 128256 bf16 logits: top-k 50 + top-p 0.9 21 us for one
-// row and 33 us for 64; top-p 0.9 alone 37 and 72 us; no filter 12 and 28 us;
+// Measured per call at 128256 bf16 logits: top-k 50 + top-p 0.9 17 us for one
+// row and 27 us for 64; top-p 0.9 alone 31 and 54 us; no filter 10 and 20 us;
 // greedy 4 and 7 us.  A row alone is bound by the latency of its phases (about
 // a microsecond per cluster barrier with the sums around it); 64 rows by the
-// fp64 exponentials, 0.5 clocks per SM and token.
+// issue of their passes, two CTAs a row: weights 10 us (45 instructions a token,
+// 8 of them fp64), counts by distance 12 us (two shared-memory atomics), weights
+// with the list of the last bin 16 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -108,7 +110,7 @@ struct Work {
     uint32_t best_at;
     float cta_best;       // of this CTA, read by the cluster
     uint32_t cta_best_at;
-    uint32_t listed;      // rank 0: entries of the list
+    uint32_t listed;      // entries of this CTA's list
     uint32_t kth, cut;    // written by rank 0
     uint64_t bin_mass;
     unsigned long long part[kWarps];
@@ -116,31 +118,39 @@ struct Work {
     uint64_t before;
 };
 // In the place of the count descent's bins: this CTA's counts and masses of
-// the first pass, later (rank 0) the list of one bin's tokens.
+// the first pass, later the list of one bin's tokens.
 struct Bins {
     uint32_t count[kBins];
-    unsigned long long mass[kBins];
+    union {
+        unsigned long long mass[kBins];
+        uint32_t place[kBins];
+    };
 };
 static_assert(sizeof(Bins) <= sizeof(Shared::hist), "room for the bins");
 
-// w * 2^S as an integer.
+// w * 2^S as an integer.  With y = (x - M) log2(e) / T, -62 < y <= 0, one product adds y to 192 + 2^-10, whose last
+// bit is 2^-45: the sum's bits are, from the top, floor(y') + 64 (y' = y + 2^-10), the first 9 bits behind the point
+// and the rest, from which 2^-10 is taken off again: |f| <= 2^-10.
 struct Mass {
-    const double *tab;
-    double best, inv_t;
-    int S;
+    const double *tab;        // 2^(i / 512) 2^(S - 64)
+    double best, scale;
+    float cut;                // what lies below has w < 2^-61: nothing of it is left by the rounding to 2^-S, S <= 51
+    __device__ __forceinline__ Mass(const double *tab_, float best_, float temp) : tab(tab_), best(best_) {
+        const double t = temp < INFINITY ? (double)temp : 1e300;
+        scale = 1.442695040888963407 / t;
+        cut = __double2float_ru(best - 42.9 * t);  // finite: x = -inf lies below
+    }
     __device__ __forceinline__ uint64_t operator()(float x) const {  // the maximum itself: exactly 2^S
-        const double d = (double)x - best;
-        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the rounded integer
-        const double t = fma(d, inv_t * (kTab / 0.693147180559945309417), kMagic);
-        if (!(t > kMagic - 44.0 * 740.0)) return 0;  // w below 2^-63, and x = -inf
-        const int n = __double2loint(t);
-        // r = d / T - n ln2 / 512, |n ln2 / 512| < 45: off by 2^-47 at most
-        const double r = fma(d, inv_t, (t - kMagic) * (-0.693147180559945309417 / kTab));
-        const double p = fma(r, fma(r, fma(r, 1.0 / 6.0, 0.5), 1.0), 1.0);
-        const double w = p * tab[n & (kTab - 1)];  // 1 <= w < 2.002
-        // 2^S * 2^(n div 512) enters through the exponent; the rounding to an integer by adding 2^52
-        const double scaled = __hiloint2double(__double2hiint(w) + ((S + (n >> 9)) << 20), __double2loint(w));
-        return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
+        const double d = (double)x - best, at = fma(d, scale, 192.0 + 1.0 / 1024.0);
+        const double y = x >= cut ? at : 130.0;  // (2^-62)
+        const int hi = __double2hiint(y);
+        const double f = __hiloint2double((hi & 0xf) | 0x40600000, __double2loint(y)) - (128.0 + 1.0 / 1024.0);
+        constexpr double c1 = 0.693147180559945309, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;  // 2^f = e^(f ln 2)
+        const double p = fma(f, fma(f, fma(f, c3, c2), c1), 1.0);
+        const double t = tab[(hi >> 4) & (kTab - 1)];
+        // the exponent of w by addition; adding 2^52 rounds the product to an integer
+        const double w = __hiloint2double(__double2hiint(t) + ((hi & 0xfe000) << 7), __double2loint(t));
+        return (uint64_t)__double_as_longlong(fma(p, w, 4503599627370496.0)) & 0xfffffffffffffull;
     }
 };
 
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     cg::cluster_group cl = cg::this_cluster();
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / C;
-    for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab);
+    for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab + (double)(a.S - 64));
     if (tid == 0) wk.listed = 0;
     pdl_trigger();
     pdl_wait();
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         best = 0.0f;
     }
     if (kCached) __syncthreads();  // the slice as the other threads read it from here on
-    const Mass mass{wk.tab, (double)best, 1.0 / (double)temp, a.S};
+    const Mass mass(wk.tab, best, temp);
 
     // What is kept so far: keys above `kth`, equal ones below the row position `cut`.
     uint32_t kth = 0, cut = 0xffffffffu;
@@ -381,7 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             constexpr bool kMass = decltype(what)::value == kMassToo, kPlaced = decltype(what)::value == kPlace;
             for (int i = tid; i < kBins; i += kThreads) {
                 bins.count[i] = 0;
-                if (kMass || kPlaced) bins.mass[i] = 0;
+                if (kMass) bins.mass[i] = 0;
+                if (kPlaced) bins.place[i] = 0;
             }
             __syncthreads();
             // everything far below goes to the last bin: added up per thread first
@@ -398,10 +409,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                     const int b = (int)d;
                     atomicAdd(&bins.count[b], 1u);
                     if (kMass) atomicAdd(&bins.mass[b], (unsigned long long)w);
-                    // the low half of the bin's 64 bits: at most 2^20 tokens, fewer than 2^10 places each
+                    // at most 2^20 tokens, fewer than 2^10 places each
                     if (kPlaced) {
                         const float fb = __int_as_float(0x4b000000 | b) - 8388608.0f;  // (float)b
-                        atomicAdd(reinterpret_cast<uint32_t *>(&bins.mass[b]), (uint32_t)((d - fb) * kPlaces));
+                        atomicAdd(&bins.place[b], (uint32_t)((d - fb) * kPlaces));
                     }
                 }
             }
@@ -416,45 +427,70 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             }
             cl.sync();
             cluster_share(cl, bins.count, wk.tot_count);
-            if (kMass || kPlaced) cluster_share(cl, bins.mass, wk.tot_mass);
+            if (kMass) cluster_share(cl, bins.mass, wk.tot_mass);
+            if (kPlaced) cluster_share(cl, bins.place, wk.tot_mass);
             share_sums(sh.cross, cl, wk.tot_count, sh.warp64);  // its barrier: the bins' place is free
         };
-        // Puts the kept ones of a warp's elements into rank 0's list (room for kList) as (key, ~row position).
-        auto append = [&](bool hit, int i) {
-            const uint32_t kx = hit ? value_key<T>(load(i)) : 0;
-            hit = hit && keep(kx, i);
-            const uint32_t m = __ballot_sync(0xffffffffu, hit);
-            if (!m) return;
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(of_rank(cl, &wk.listed, 0), (uint32_t)__popc(m));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1u));
-            if (hit && at < kList) of_rank(cl, list, 0)[at] = ((unsigned long long)kx << 32) | (uint32_t)~(uint32_t)(base + i);
+        // Puts the kept ones of a warp's elements as (key, ~row position) into the CTA's list (room for kList) or,
+        // when few are expected, into rank 0's, which saves join_lists' barrier.
+        unsigned long long *list_to = list;
+        uint32_t *listed_to = &wk.listed;
+        auto straight_to_rank0 = [&](uint32_t expected) {  // at most `expected` entries in all; cluster-uniform
+            const bool yes = expected <= 512;
+            list_to = yes ? of_rank(cl, list, 0) : list;
+            listed_to = yes ? of_rank(cl, &wk.listed, 0) : &wk.listed;
+            return yes;
         };
-        // Waits for the list and sorts it in rank 0, descending.  Returns its length.
-        auto sorted = [&]() {
-            cl.sync();
-            const int m = min((int)wk.listed, kList);
-            if (rank == 0) sort_descending(list, m);
-            return m;
-        };
-        // The kept tokens of bins b0 .. b1 in the list, sorted.
-        auto gather = [&](int b0, int b1) {
-            const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
-            constexpr int kTake = 4;
-            for (int i0 = warp * 32; i0 < n; i0 += kThreads * kTake) {
-                bool hit[kTake], any = false;
-#pragma unroll
-                for (int q = 0; q < kTake; ++q) {
-                    const int i = i0 + q * kThreads + lane;
-                    const float d = i < n ? distance(load(i)) : -1.0f;
-                    hit[q] = !(d < d0) && !(d >= d1);
-                    any = any || hit[q];
+        // A lane's elements come as bits: bit j for element first + j step.
+        auto append = [&](uint32_t mask, int first, int step) {
+            if (kth != 0) {  // cluster-uniform
+                for (uint32_t m = mask; m; m &= m - 1) {
+                    const int i = first + (__ffs(m) - 1) * step;
+                    if (!keep(value_key<T>(load(i)), i)) mask &= ~(m & -m);
                 }
-                if (!__any_sync(0xffffffffu, any)) continue;
-#pragma unroll
-                for (int q = 0; q < kTake; ++q) append(hit[q], i0 + q * kThreads + lane);
             }
-            return sorted();
+            if (!__any_sync(0xffffffffu, mask)) return;
+            const uint32_t c = __popc(mask);
+            uint32_t upto = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            uint32_t at = 0;
+            if (lane == 31) at = atomicAdd(listed_to, upto);
+            at = __shfl_sync(0xffffffffu, at, 31) + upto - c;
+            for (; mask; mask &= mask - 1, ++at) {
+                const int i = first + (__ffs(mask) - 1) * step;
+                if (at < kList) list_to[at] = ((unsigned long long)value_key<T>(load(i)) << 32) | (uint32_t)~(uint32_t)(base + i);
+            }
+        };
+        // After a cluster barrier: brings the lists to rank 0 and sorts them there, descending.  Returns how
+        // many entries there are; more than kList: no list.
+        auto sorted = [&](bool at_rank0) {
+            const int m = at_rank0 ? (int)wk.listed : (int)join_lists(cl, list, &wk.listed);
+            if (rank == 0 && m <= kList) sort_descending(list, m);
+            return m;  // at_rank0: known there
+        };
+        // The kept tokens of bins b0 .. b1, at most `expected`, in rank 0's list, sorted.  Returns their number there.
+        auto gather = [&](int b0, int b1, uint32_t expected) {
+            const bool at_rank0 = straight_to_rank0(expected);
+            const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
+            for (int i0 = warp * 32; i0 < n; i0 += kThreads * 32) {
+                uint32_t mask = 0;
+                for (int j = 0; j < 32 && i0 + j * kThreads < n; j += 2) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int i = i0 + (j + q) * kThreads + lane;
+                        const float d = i < n ? distance(load(i)) : -1.0f;
+                        const bool hit = !(d < d0) & !(d >= d1);
+                        mask |= (uint32_t)hit << (j + q);
+                    }
+                }
+                append(mask, i0 + lane, kThreads);
+            }
+            cl.sync();
+            return min(sorted(at_rank0), kList);
         };
         auto listed_mass = [&](int i) { return mass(key_value<T>((uint32_t)(list[i] >> 32))); };
         // Rank 0's finding reaches the cluster; the list is free again.
@@ -476,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             at_k = crossing(sh.cross, cl, wk.tot_count, (uint64_t)k, sh.warp64);
             if (at_k.before + at_k.here <= kList) {
                 // everything that may be kept fits the list: rank 0 finishes alone
-                gather(0, (int)at_k.slot);
+                gather(0, (int)at_k.slot, (uint32_t)(at_k.before + at_k.here));
                 if (rank != 0) return;  // nobody reads the other CTAs' shared memory any more
                 int kept = k;
                 if (by_mass || least > 0) {
@@ -542,36 +578,34 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             __syncthreads();
             const uint64_t about = share_sums(sh.cross, cl, wk.tot_mass, sh.warp64);
             const uint64_t slack = about / 8192, aim = want_of(about);
-            const Crossing from = crossing(sh.cross, cl, wk.tot_mass, aim > slack ? aim - slack : 1, sh.warp64);
-            cl.sync();  // every CTA has its copy; the second search starts from the same sums
-            const Crossing to = crossing(sh.cross, cl, wk.tot_mass, min(aim + slack, about), sh.warp64);
-            const int b0 = (int)from.slot, b1 = aim + slack < about ? (int)to.slot : kBins - 1;
+            const uint64_t ends[2] = {aim > slack ? aim - slack : 1, min(aim + slack, about)};
+            Crossing at[2];
+            crossings(sh.cross, cl, wk.tot_mass, ends, at, sh.warp64);
+            const int b0 = (int)at[0].slot, b1 = ends[1] < about ? (int)at[1].slot : kBins - 1;
             {
-                const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : __int_as_float(0x7fc00000);
+                const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : 3e38f;  // (what lies further off has no mass)
                 int lo, hi;
                 warp_part(n, lo, hi);
-                uint64_t rest = 0, above = 0, part = 0;
-                constexpr int kTake = 4;
+                uint64_t all = 0, above = 0, part = 0;
                 auto add_up = [&](auto by_min) {  // with min-p the kept masses are not all of those above
-                    for (int i0 = lo; i0 < hi; i0 += 32 * kTake) {
-                        bool hit[kTake], any = false;
+                    for (int i0 = lo; i0 < hi; i0 += 32 * 32) {
+                        uint32_t mask = 0;
+                        for (int j = 0; j < 32 && i0 + 32 * j < hi; j += 4) {
 #pragma unroll
-                        for (int q = 0; q < kTake; ++q) {
-                            const int i = i0 + 32 * q + lane;
-                            const float x = i < hi ? load(i) : -INFINITY, d = distance(x);
-                            const uint64_t w = mass(x);
-                            if (d < d0) {
-                                above += w;
-                                if (decltype(by_min)::value) part += w >= least ? w : 0;
-                            } else {
-                                rest += w;
+                            for (int q = 0; q < 4; ++q) {
+                                const int i = i0 + 32 * (j + q) + lane;
+                                const float x = i < hi ? load(i) : -INFINITY, d = distance(x);
+                                const uint64_t w = mass(x);
+                                all += w;
+                                const bool stays = d < d0;
+                                const uint64_t kept = stays ? w : 0;
+                                above += kept;
+                                if (decltype(by_min)::value) part += kept >= least ? kept : 0;
+                                const bool hit = !stays & (d < d1);
+                                mask |= (uint32_t)hit << (j + q);
                             }
-                            hit[q] = i < hi && !(d < d0) && !(d >= d1);
-                            any = any || hit[q];
                         }
-                        if (!__any_sync(0xffffffffu, any)) continue;
-#pragma unroll
-                        for (int q = 0; q < kTake; ++q) append(hit[q], i0 + 32 * q + lane);
+                        append(mask, i0 + lane, 32);
                     }
                 };
                 if (least > 0) {
@@ -583,21 +617,21 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
                 if (lane == 0) wk.part[warp] = part;
-                const ulonglong2 sums = cluster_sum2(sh, cl, rest, above);
-                const uint64_t want = want_of(sums.x + sums.y);
+                const ulonglong2 sums = cluster_sum2(sh, cl, all, above);
+                const uint64_t want = want_of(sums.x);
                 above = sums.y;
-                const int m = sorted();
+                const int m = sorted(false);  // (cluster_sum2 ended with a barrier)
                 if (rank == 0) {
                     if (tid == 0) for (int r = 0; r < C; ++r) *of_rank(cl, &wk.kth, r) = 0;
                     __syncthreads();
                     // the part of a row position: its CTA's slice, its warp's share of the slice
                     uint64_t before = above;
-                    for (int i0 = 0; i0 < m; i0 += kThreads) {  // block-uniform
+                    for (int i0 = 0; i0 < m && m <= kList; i0 += kThreads) {  // block-uniform
                         const int i = i0 + tid;
                         const uint64_t w = i < m ? listed_mass(i) : 0;
                         uint64_t sum;
                         const uint64_t mine = before + block_exclusive(w, sh.warp64, &sum);
-                        if (i < m && mine < want && wk.listed <= kList) {
+                        if (i < m && mine < want) {
                             if (want <= mine + w) publish(list[i]);
                             if (w >= least) {
                                 const int at = (int)~(uint32_t)list[i], r = at / a.slice;
@@ -619,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             const uint32_t rest = (uint32_t)k - (uint32_t)at_k.before;
             uint64_t dropped = 0;
             if (at_k.here <= kList) {
-                const int m = gather(b, b);
+                const int m = gather(b, b, (uint32_t)at_k.here);
                 if (rank == 0) {
                     if (tid == 0) publish(list[(rest - 1) & (kList - 1)]);
                     uint64_t mine = 0;
@@ -657,8 +691,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             const uint64_t want = want_of(share_sums(sh.cross, cl, wk.tot_mass, sh.warp64));
             const Crossing at = crossing(sh.cross, cl, wk.tot_mass, want, sh.warp64);
             const int b = (int)at.slot, W = kBins / C;
-            if (*of_rank(cl, wk.tot_count + b % W, b / W) <= kList) {
-                const int m = gather(b, b);
+            const uint32_t count = *of_rank(cl, wk.tot_count + b % W, b / W);
+            if (count <= kList) {
+                const int m = gather(b, b, count);
                 if (rank == 0) {
                     uint64_t before = at.before;
                     for (int i0 = 0; i0 < m; i0 += kThreads) {  // block-uniform
@@ -695,8 +730,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     if (parts_known) {
         part = wk.part[warp];
     } else {
+        if (kth == 0 && least == 0) {  // everything is kept
 #pragma unroll 4
-        for (int i = lo + lane; i < hi; i += 32) part += kept_mass(i);
+            for (int i = lo + lane; i < hi; i += 32) part += mass(load(i));
+        } else {
+#pragma unroll 4
+            for (int i = lo + lane; i < hi; i += 32) part += kept_mass(i);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     }

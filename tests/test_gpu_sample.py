@@ -151,6 +151,16 @@ def test_sample_extreme_numbers():
     assert 0 <= int(tok[5]) < 333
 
 
+@pytest.mark.parametrize("scale", [1.0, 1e30])
+@pytest.mark.parametrize("T", [1e-30, 1e-3, 1e30, 3e38, float("inf")])
+def test_sample_extreme_temperatures(T, scale):
+    x, u = rows(4, 2500, "fp32", seed=5)
+    x *= scale
+    x[1, 3] = torch.finfo(x.dtype).min  # finite: as likely as any other when the temperature is infinite
+    for s in (dict(), dict(k=2000), dict(p=0.7), dict(mp=0.5), dict(k=400, p=0.3)):
+        check(x, u, T=T, **s)
+
+
 def test_sample_distribution():
     """Evenly spaced numbers draw every token in proportion to its probability, to one part in their count."""
     import custom_ecc_cuda as ops
