@@ -334,49 +334,82 @@ static inline int cluster_size(void (*kernel)(KArgs...), int64_t clusters, int64
     return c;
 }
 
-// Descending bitonic sort of the first n entries of `x` by the whole block; the
-// entries from n up to the next power of two (at least 32) are overwritten.  Up
-// to 1024 entries a thread holds one: partners within a warp are exchanged by
-// shuffles, only strides of 32 and more go through shared memory, and only the
-// warps that hold entries meet at those barriers (64 entries: 0.5 us, where a
-// block barrier per stride took 3).
-__device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
-    int size = 32;
-    while (size < n) size *= 2;
-    const int t = threadIdx.x;
-    if (size <= kThreads) {
-        if (t < size) {
-            unsigned long long v = t < n ? x[t] : 0ull;
-            for (int k = 2; k <= size; k *= 2)
-                for (int j = k / 2; j > 0; j /= 2) {
-                    unsigned long long u;
-                    if (j < 32) {
-                        u = __shfl_xor_sync(0xffffffffu, v, j);
-                    } else {
-                        asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");  // earlier readers are done
-                        x[t] = v;
-                        asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");
-                        u = x[t ^ j];
-                    }
-                    v = (((t & j) == 0) == ((t & k) == 0)) == (v < u) ? u : v;
-                }
-            asm volatile("bar.sync 2, %0;" ::"r"(size) : "memory");
-            x[t] = v;
-        }
-        __syncthreads();
-        return;
-    }
-    for (int i = n + t; i < size; i += kThreads) x[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
+// Bitonic sort of `size` entries, a power of two from 32 E to 1024 E, by size /
+// E threads that hold E neighbouring entries each (0 behind entry n).  Partners
+// in a thread are exchanged in registers, those in a warp by shuffles; strides
+// of 32 E and more go through shared memory.
+template <int E>
+__device__ __forceinline__ void sort_bitonic(unsigned long long *x, int n, int size) {
+    const int t = threadIdx.x, threads = size / E;
+    if (t >= threads) return;
+    unsigned long long v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = t * E + e < n ? x[t * E + e] : 0ull;
+    for (int k = 2; k <= size; k *= 2) {
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int p = t; p < size / 2; p += kThreads) {
-                const int i = 2 * p - (p & (j - 1));  // bit j of i is clear
-                const unsigned long long a = x[i], b = x[i + j];
-                if ((a < b) == ((i & k) == 0)) x[i] = b, x[i + j] = a;
+            if (j < E) {
+#pragma unroll
+                for (int s = E / 2; s > 0; s /= 2) {
+                    if (j != s) continue;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (e & s) continue;
+                        const unsigned long long p = v[e], q = v[e + s];
+                        const bool swap = (p < q) == (((t * E + e) & k) == 0);
+                        v[e] = swap ? q : p;
+                        v[e + s] = swap ? p : q;
+                    }
+                }
+                continue;
             }
-            __syncthreads();
+            const int w = j / E;  // in threads
+            const bool larger = ((t & w) == 0) == ((t * E & k) == 0);  // (k > j >= E)
+            unsigned long long u[E];
+            if (w < 32) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] = __shfl_xor_sync(0xffffffffu, v[e], w);
+            } else {
+                asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");  // earlier readers are done
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[t * E + e] = v[e];
+                asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+#pragma unroll
+                for (int e = 0; e < E; ++e) u[e] = x[(t ^ w) * E + e];
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = larger == (v[e] < u[e]) ? u[e] : v[e];
         }
+    }
+    asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[t * E + e] = v[e];
+}
+
+// Descending sort of the first n <= 4096 entries of `x`, all different, by the
+// whole block; entries from n up to the next power of two may be overwritten.
+// Up to 128 an entry's place is the number of larger ones, counted by 8 to 32
+// threads (100: 1.0 us, by exchanges 1.6); more are sorted by exchanges: 500 in
+// 3.6 us, 1000 in 6.8, 4096 in 23 (by merges of ranked runs 2.9, 5.7 and 26).
+__device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
+    const int t = threadIdx.x;
+    if (n <= 128) {
+        const int lg = n <= 32 ? 5 : n <= 64 ? 4 : 3;  // 2^lg threads an entry
+        const int i = t >> lg, each = 1 << lg, threads = ((n << lg) + 31) / 32 * 32;
+        if (t < threads) {
+            const unsigned long long v = i < n ? x[i] : 0ull;
+            int larger = 0;
+            for (int q = t & (each - 1); q < n; q += each) larger += x[q] > v ? 1 : 0;
+            for (int o = 1; o < each; o *= 2) larger += __shfl_xor_sync(0xffffffffu, larger, o);
+            asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+            if (i < n && (t & (each - 1)) == 0) x[larger] = v;
+        }
+    } else {
+        int size = 256;
+        while (size < n) size *= 2;
+        if (size <= 512) sort_bitonic<1>(x, n, size);
+        else sort_bitonic<4>(x, n, size);
+    }
+    __syncthreads();
 }
 
 // Launch with a cluster of `c` CTAs per row (y), as a dependent of the kernel

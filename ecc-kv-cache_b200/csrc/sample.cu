@@ -26,7 +26,7 @@
 // of the exponential function, 1989).
 //
 // Measured per call at 128256 bf16 logits: top-k 50 + top-p 0.9 17 us for one
-// row and 27 us for 64; top-p 0.9 alone 31 and 54 us; no filter 10 and 20 us;
+// row and 26 us for 64; top-p 0.9 alone 31 and 55 us; no filter 10 and 20 us;
 // greedy 4 and 7 us.  A row alone is bound by the latency of its phases (about
 // a microsecond per cluster barrier with the sums around it); 64 rows by the
 // issue of their passes, two CTAs a row: weights 10 us (45 instructions a token,
