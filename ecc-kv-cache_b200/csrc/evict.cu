@@ -13,7 +13,7 @@
 // Measured at 8 sequences x 8 kv heads, 32768 -> 16384 tokens: selection 26 us
 // (5 reading the weights, 5 writing positions and weights, the rest the
 // barriers of its phases), move 87 us, 6.1 TB/s of the 0.54 GB read and written
-// (bound by memory).  One sequence of 5001 tokens to 1024: 14 + 3 us; three
+// (bound by memory).  One sequence of 5001 tokens to 1024: 15 + 3 us; three
 // digit descents instead of the binned pass took 24 + 5.
 #include <algorithm>
 
