@@ -432,17 +432,23 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
     const int tid = threadIdx.x, d = tid & (kD - 1), grp = tid / kD, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
     pdl_wait();
-    const int len = seq_len_of(a, b);
+    // a short context is a chain of loads: each is asked for as early as its address is known
+    const int len = seq_len_of(a, b), first = a.row_first[row], last = a.row_last[row];
     int n = 0;
     int64_t base = 0;
     if (len > 0) {  // an empty sequence has no partials
-        const int first = a.row_first[row];
-        n = min(a.row_last[row] - first + 1, kMaxRanges);
+        n = min(last - first + 1, kMaxRanges);
         base = (int64_t)first + row;
         // lengths that changed between the two kernels must not lead out of the workspace
         if (first < 0 || base + n > a.slots) n = 0, base = 0;
     }
     const float *pm = a.pm + base * G + e, *pl = a.pl + base * G + e, *po = a.po + (base * G + e) * kD + d;
+    constexpr int kEarly = 8;
+    float early[kEarly];
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+        early[k] = grp + k * kMergeGroups < n ? po[(int64_t)(grp + k * kMergeGroups) * G * kD] : 0.0f;
+    const float early_l = tid < n ? pl[(int64_t)tid * G] : 0.0f;
     float mx = -INFINITY;
     for (int i = tid; i < n; i += kD * kMergeGroups) {
         const float m = pm[(int64_t)i * G];
@@ -460,7 +466,7 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
     for (int i = tid; i < n; i += kD * kMergeGroups) {  // the entries this thread wrote
         const float w = M == -INFINITY ? 0.0f : exp2f(s_w[i] - M);
         s_w[i] = w;
-        ls = fmaf(pl[(int64_t)i * G], w, ls);
+        ls = fmaf(i == tid ? early_l : pl[(int64_t)i * G], w, ls);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
@@ -471,8 +477,11 @@ paged_merge_kernel(const __grid_constant__ DecodeArgs a, __half *__restrict__ ou
     for (int k = 0; k < kD * kMergeGroups / 32; ++k) Ls += s_red[1][k];
 
     float acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k)
+        if (grp + k * kMergeGroups < n) acc = fmaf(early[k], s_w[grp + k * kMergeGroups], acc);
 #pragma unroll 8
-    for (int i = grp; i < n; i += kMergeGroups) acc = fmaf(po[(int64_t)i * G * kD], s_w[i], acc);
+    for (int i = grp + kEarly * kMergeGroups; i < n; i += kMergeGroups) acc = fmaf(po[(int64_t)i * G * kD], s_w[i], acc);
     s_o[grp][d] = acc;
     __syncthreads();
     if (grp == 0) {
