@@ -176,13 +176,17 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     __syncthreads();
 
     const int Hkv = a.Hkv;
-    const int64_t T = (int64_t)s_pre[a.B] * Hkv;
-    const int64_t NW = min((int64_t)gridDim.x * kWarps, T);
+    const uint32_t T = (uint32_t)s_pre[a.B] * Hkv;  // below 2^31 (check_shape)
+    const uint32_t NW = min(gridDim.x * kWarps, T);
     // neighbouring ranges go to different SMs: a few tiles spread over the GPU
     const int64_t wid = (int64_t)warp * gridDim.x + blockIdx.x;
     if (wid >= NW) return;
-    const int64_t tbeg = wid * T / NW;
-    const int ntiles = (int)((wid + 1) * T / NW - tbeg);
+    const uint32_t w32 = (uint32_t)wid;
+    // range w starts at tile floor(w T / NW): with T = q NW + r that is w q + floor(w r / NW), w r < 2^24
+    const uint32_t q_tiles = T / NW, r_tiles = T - q_tiles * NW;
+    static_assert(kMaxRanges <= 4096, "products below 2^24");
+    const int64_t tbeg = (int64_t)(w32 * q_tiles + w32 * r_tiles / NW);
+    const int ntiles = (int)((int64_t)((w32 + 1) * q_tiles + (w32 + 1) * r_tiles / NW) - tbeg);
 
     // a sequence's tiles; their number is the one that the cut was made with
     auto tiles_of = [&](int b) {
