@@ -27,6 +27,25 @@ constexpr int kCopies = 4;
 constexpr int kPerThread = kBins / kThreads;
 constexpr int kMaxCluster = 16;
 
+// The cluster of this CTA; one of a single CTA meets at the block's barrier.
+class Cluster {
+    int n_, rank_;
+
+public:
+    __device__ __forceinline__ Cluster()
+        : n_((int)cg::this_cluster().num_blocks()), rank_((int)cg::this_cluster().block_rank()) {}
+    __device__ __forceinline__ int num_blocks() const { return n_; }
+    __device__ __forceinline__ int block_rank() const { return rank_; }
+    __device__ __forceinline__ void sync() const {
+        if (n_ == 1) __syncthreads();
+        else cg::this_cluster().sync();
+    }
+    template <class T>
+    __device__ __forceinline__ T *map_shared_rank(T *p, unsigned rank) const {
+        return cg::this_cluster().map_shared_rank(p, rank);
+    }
+};
+
 struct Crossing {  // see crossing()
     uint32_t slot;
     uint64_t before, here;
@@ -56,7 +75,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 
 template <class T>
-__device__ __forceinline__ T *of_rank(cg::cluster_group &cl, T *p, unsigned rank) {
+__device__ __forceinline__ T *of_rank(const Cluster &cl, T *p, unsigned rank) {
     return cl.map_shared_rank(p, rank);
 }
 
@@ -92,7 +111,7 @@ __device__ __forceinline__ T block_exclusive(T v, T *warp_sums, T *total) {
 // cluster barrier since their `from` was written, and pass one (crossing()
 // does) before it is written again.
 template <class T, class U>
-__device__ __forceinline__ void cluster_share(cg::cluster_group &cl, T *from, U *to) {
+__device__ __forceinline__ void cluster_share(const Cluster &cl, T *from, U *to) {
     const int ranks = (int)cl.num_blocks(), W = kBins / ranks, at = (int)cl.block_rank() * W;
     for (int i = threadIdx.x; i < W; i += kThreads) {
         T c = 0;
@@ -110,7 +129,7 @@ __device__ __forceinline__ void cluster_share(cg::cluster_group &cl, T *from, U 
 
 // The sum of all bins; every CTA's cs.share is filled.
 template <class T>
-__device__ __forceinline__ uint64_t share_sums(CrossingShared &cs, cg::cluster_group &cl, const T *bins,
+__device__ __forceinline__ uint64_t share_sums(CrossingShared &cs, const Cluster &cl, const T *bins,
                                                uint64_t *warp_sums) {
     const int ranks = (int)cl.num_blocks(), W = kBins / ranks;
     uint64_t v = 0;
@@ -127,7 +146,7 @@ __device__ __forceinline__ uint64_t share_sums(CrossingShared &cs, cg::cluster_g
 // reaches want[j] (1 <= want[j] <= the sum of all): the bin, the sum before it
 // and its own, the same in every CTA.  Ends with a cluster barrier.
 template <class T, int K>
-__device__ __forceinline__ void crossings(CrossingShared &cs, cg::cluster_group &cl, const T *bins,
+__device__ __forceinline__ void crossings(CrossingShared &cs, const Cluster &cl, const T *bins,
                                           const uint64_t (&want)[K], Crossing (&found)[K], uint64_t *warp_sums) {
     const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank(), W = kBins / ranks;
     uint64_t before = 0;
@@ -165,7 +184,7 @@ __device__ __forceinline__ void crossings(CrossingShared &cs, cg::cluster_group 
     }
 }
 template <class T>
-__device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_group &cl, const T *bins, uint64_t want,
+__device__ __forceinline__ Crossing crossing(CrossingShared &cs, const Cluster &cl, const T *bins, uint64_t want,
                                              uint64_t *warp_sums) {
     const uint64_t w[1] = {want};
     Crossing f[1];
@@ -178,7 +197,7 @@ __device__ __forceinline__ Crossing crossing(CrossingShared &cs, cg::cluster_gro
 // bit `low` (the bits below are zero in every key).  *ties: how many of the
 // keys equal to it belong to the k largest; *equal: how many there are.
 template <class Keys>
-__device__ __forceinline__ uint32_t kth_largest(Shared &sh, cg::cluster_group &cl, const Keys &keys, int n, uint32_t k,
+__device__ __forceinline__ uint32_t kth_largest(Shared &sh, const Cluster &cl, const Keys &keys, int n, uint32_t k,
                                                 int low, uint32_t *ties, uint32_t *equal) {
     const int tid = threadIdx.x;
     const unsigned ranks = cl.num_blocks();
@@ -233,7 +252,7 @@ __device__ __forceinline__ uint32_t warp_count(int lo, int hi, const Pred &p) {
 }
 
 // Cluster-wide exclusive prefix of one count per warp, in row order.
-__device__ __forceinline__ uint32_t cluster_exclusive(Shared &sh, cg::cluster_group &cl, uint32_t warp_value) {
+__device__ __forceinline__ uint32_t cluster_exclusive(Shared &sh, const Cluster &cl, uint32_t warp_value) {
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = warp_value;
     __syncthreads();
@@ -250,7 +269,7 @@ __device__ __forceinline__ uint32_t cluster_exclusive(Shared &sh, cg::cluster_gr
 // p(i): elements of equal key are kept below it.  base: row position of this
 // CTA's element 0.
 template <class Pred>
-__device__ __forceinline__ uint32_t tie_cut(Shared &sh, cg::cluster_group &cl, int n, int base, uint32_t ties,
+__device__ __forceinline__ uint32_t tie_cut(Shared &sh, const Cluster &cl, int n, int base, uint32_t ties,
                                             const Pred &p) {
     int lo, hi;
     warp_part(n, lo, hi);
@@ -280,7 +299,7 @@ constexpr int kList = sizeof(Shared::hist) / 8;
 // number in *listed) behind one another into the first CTA's.  All CTAs have
 // passed a cluster barrier since their last entry; ends with one.  Returns the
 // number of all entries; nothing is moved when that is more than kList.
-__device__ __forceinline__ uint32_t join_lists(cg::cluster_group &cl, unsigned long long *list, const uint32_t *listed) {
+__device__ __forceinline__ uint32_t join_lists(const Cluster &cl, unsigned long long *list, const uint32_t *listed) {
     const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     uint32_t before = 0, mine = 0, all = 0;
     for (int r = 0; r < ranks; ++r) {

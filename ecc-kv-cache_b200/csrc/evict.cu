@@ -13,7 +13,7 @@
 // Measured at 8 sequences x 8 kv heads, 32768 -> 16384 tokens: selection 26 us
 // (5 reading the weights, 5 writing positions and weights, the rest the
 // barriers of its phases), move 87 us, 6.1 TB/s of the 0.54 GB read and written
-// (bound by memory).  One sequence of 5001 tokens to 1024: 15 + 3 us; three
+// (bound by memory).  One sequence of 5001 tokens to 1024: 12 + 3 us; three
 // digit descents instead of the binned pass took 24 + 5.
 #include <algorithm>
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);  // the NaN key gives a NaN
 }
 
-__device__ void check_tables(const EvictArgs &a, sel::cg::cluster_group &cl) {
+__device__ void check_tables(const EvictArgs &a, const sel::Cluster &cl) {
     const int t0 = cl.block_rank() * sel::kThreads + threadIdx.x, step = cl.num_blocks() * sel::kThreads;
     for (int i = t0; i < (a.src.n_pages + 31) / 32; i += step) a.bitmap[i] = 0;
     if (t0 == 0) *a.clash = 0;
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(sel::kThreads, 1) evict_select_kernel(const __
     extern __shared__ __align__(16) uint8_t dyn[];
     sel::Shared &sh = *reinterpret_cast<sel::Shared *>(dyn);
     uint32_t *cache = reinterpret_cast<uint32_t *>(dyn + sizeof(sel::Shared));
-    sel::cg::cluster_group cl = sel::cg::this_cluster();
+    const sel::Cluster cl;
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31;
     pdl_trigger();
     pdl_wait();

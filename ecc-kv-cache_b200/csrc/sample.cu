@@ -173,7 +173,7 @@ __device__ __forceinline__ uint64_t share_of(float f, uint64_t total, bool *cut_
 }
 
 // Sum of v over the cluster's threads.
-__device__ __forceinline__ uint64_t cluster_sum(Shared &sh, cg::cluster_group &cl, uint64_t v) {
+__device__ __forceinline__ uint64_t cluster_sum(Shared &sh, const Cluster &cl, uint64_t v) {
     uint64_t all;
     block_exclusive(v, sh.warp64, &all);
     if (threadIdx.x == 0) sh.cta64 = all;
@@ -185,7 +185,7 @@ __device__ __forceinline__ uint64_t cluster_sum(Shared &sh, cg::cluster_group &c
 }
 
 // Two sums at once: a pair per CTA in the first CTAs' entries of `share`.
-__device__ __forceinline__ ulonglong2 cluster_sum2(Shared &sh, cg::cluster_group &cl, uint64_t x, uint64_t y) {
+__device__ __forceinline__ ulonglong2 cluster_sum2(Shared &sh, const Cluster &cl, uint64_t x, uint64_t y) {
     static_assert(kMaxCluster >= 16, "two entries for each of 8 CTAs");
     const int ranks = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     uint64_t ax, ay;
@@ -209,7 +209,7 @@ __device__ __forceinline__ ulonglong2 cluster_sum2(Shared &sh, cg::cluster_group
 template <class T, class Load, class Keep, class BinOf>
 __device__ __noinline__ uint2 mass_descent(Shared &sh, Load load, Keep keep, BinOf bin_of, Mass mass, int n, int base,
                                            int bin, uint64_t above, uint64_t want, uint32_t kth, uint32_t cut) {
-    cg::cluster_group cl = cg::this_cluster();
+    const Cluster cl;
     unsigned long long *from = reinterpret_cast<unsigned long long *>(sh.hist), *to = from + kBins;
     const int tid = threadIdx.x, low = key_low<T>();
     uint32_t prefix = 0, mask = 0;
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     Work &wk = *reinterpret_cast<Work *>(dyn);
     Shared &sh = wk.sel;
     T *x_s = reinterpret_cast<T *>(dyn + (sizeof(Work) + 15) / 16 * 16);
-    cg::cluster_group cl = cg::this_cluster();
+    const Cluster cl;
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / C;
     for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab + (double)(a.S - 64));
