@@ -20,6 +20,7 @@ import ctypes
 import functools
 import math
 import os
+import struct
 import threading
 
 import torch
@@ -55,12 +56,6 @@ class EccError(RuntimeError):
     """A negative status from libeccb200.so."""
 
 
-class _Pages(ctypes.Structure):
-    """ecc_pages_t"""
-    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("width", ctypes.c_int),
-                ("page_size", ctypes.c_int), ("n_pages", ctypes.c_int64)]
-
-
 def _load():
     if not os.path.exists(library_path):
         raise ImportError(
@@ -68,7 +63,6 @@ def _load():
             f"`make -C {os.path.join(os.path.dirname(_HERE), 'csrc')}` (sm_100a)")
     lib = ctypes.CDLL(library_path)
     p, i64, i32, f32, sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
-    pg = ctypes.POINTER(_Pages)  # takes a _Pages by reference
     sig = {
         "ecc_strerror": ([i32], ctypes.c_char_p),
         "ecc_version": ([], i32),
@@ -111,16 +105,9 @@ def _load():
         "ecc_lse_gather_merge": ([p, p, p, i64, i32, i32, p, i32, i32, ctypes.c_uint32, ctypes.c_longlong, p, i32,
                                   p], i32),
         "ecc_lse_exchange_merge_dev": ([p, p, p, i64, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
-        "ecc_compress_paged": ([p, i64, i64, i64, p, i64, i64, p, i64, i64, i64, p, i64, i64, i32, i32, i64, pg, p, p,
-                                i32, p], i32),
-        "ecc_dequantize_paged": ([p, i64, i64, p, p, i64, i64, p, i32, i32, i64, pg, p, i32, p], i32),
         "ecc_decode_paged_workspace_size": ([i32, i32, i32, i64, i32], sz),
-        "ecc_decode_paged": ([p, p, p, i64, i64, pg, p, p, p, p, i64, i64, p, sz, i32, i32, i32, f32, i32, i32, i32, p],
-                             i32),
         "ecc_evict_paged_workspace_size": ([i64], sz),
-        "ecc_evict_paged": ([p, p, i64, i64, pg, p, p, i64, i64, pg, p, i64, i64, i64, p, i32, i32, i32, i32, i32, i32, p,
-                             sz, p], i32),
-        "ecc_sample": ([p, i64, i32, i32, i64, p, p, f32, p, i32, p, f32, p, f32, p, p, p], i32),
+        "ecc_call": ([i32, p], i32),
         "ecc_lse_gather_merge_dev": ([p, p, p, i64, i32, i32, p, i32, i32, p, ctypes.c_longlong, p, i32, p], i32),
     }
     for name, (args, res) in sig.items():
@@ -884,19 +871,39 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 _launch_locks = tuple(threading.Lock() for _ in range(64))  # by device
 
 
-def _launch(fn, what: str, dev: torch.device, *args) -> None:
-    """fn(*args, current stream of dev) with dev the current device.  One call
-    at a time: the launches of a call share a workspace, and those of another
-    thread on the same stream must not come between them."""
+class _Entry:
+    """An entry point of ecc_call: its number and the layout of its words (q:
+    pointers and integers, d: floats; the stream comes last)."""
+
+    def __init__(self, number: int, what: str, words: str):
+        self.number, self.what, self.pack = number, what, struct.Struct("=" + words).pack
+
+
+_COMPRESS_PAGED = _Entry(0, "compress_pair_paged", "26q")
+_DEQUANTIZE_PAGED = _Entry(1, "dequantize_paged", "19q")
+_DECODE_PAGED = _Entry(2, "decode_attention_paged", "21qd4q")
+_EVICT_PAGED = _Entry(3, "evict_paged", "32q")
+_SAMPLE = _Entry(4, "sample_tokens", "7qd3qdqd3q")
+
+
+def _launch(entry: _Entry, dev: torch.device, *args) -> None:
+    """The entry point with these arguments and the current stream of dev, with
+    dev the current device.  One call at a time: the launches of a call share a
+    workspace, and those of another thread on the same stream must not come
+    between them."""
     i = dev.index
+    try:
+        words = entry.pack(*args, torch._C._cuda_getCurrentRawStream(i))
+    except struct.error as e:
+        raise RuntimeError(f"{entry.what}: an argument is no number or out of range ({e})") from e
     if torch.cuda.current_device() == i:
         with _launch_locks[i & 63]:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = _lib.ecc_call(entry.number, words)
     else:
         with torch.cuda.device(dev), _launch_locks[i & 63]:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = _lib.ecc_call(entry.number, words)
     if rc:
-        _check(rc, what)
+        _check(rc, entry.what)
 
 
 def _scratch(workspace: torch.Tensor | None, dev: torch.device, need: int) -> torch.Tensor:
@@ -943,7 +950,8 @@ def _paged_pools(k_pool: torch.Tensor, v_pool: torch.Tensor | None):
     return shape, ks, vs
 
 
-def _pages(table: torch.Tensor, name: str, B: int, shape, dev: torch.device) -> _Pages:
+def _pages(table: torch.Tensor, name: str, B: int, shape, dev: torch.device) -> tuple:
+    """The five words of a page table: address, row stride, width, page size, pages."""
     if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.device != dev:
         raise RuntimeError(f"{name} must be an int32 tensor on the pools' device")
     ts = table.shape
@@ -955,7 +963,7 @@ def _pages(table: torch.Tensor, name: str, B: int, shape, dev: torch.device) -> 
         raise RuntimeError(f"{name} must have contiguous rows")
     if shape[2] % 16 and width > 1:
         raise RuntimeError(f"page_size must be a multiple of 16 (or one page per sequence), got {shape[2]}")
-    return _Pages(table.data_ptr(), row, width, shape[2], shape[0])
+    return table.data_ptr(), row, width, shape[2], shape[0]
 
 
 def _per_sequence(t: torch.Tensor, name: str, device, B: int) -> int:
@@ -1011,11 +1019,11 @@ def compress_pair_paged(k: torch.Tensor, v: torch.Tensor | None, k_pool: torch.T
         raise RuntimeError("k and v must have the pools' kv heads and 128 dimensions")
     pages = _pages(block_table, "block_table", B, shape, dev)
     pos_p = _per_sequence(pos, "pos", dev, B)
-    new_p = None if new_lens is None else _per_sequence(new_lens, "new_lens", dev, B)
+    new_p = 0 if new_lens is None else _per_sequence(new_lens, "new_lens", dev, B)
     (kb, kh, kl, _), (vb, vh, vl, _) = strides
-    _launch(_lib.ecc_compress_paged, "compress_pair_paged", dev, k.data_ptr(), kb, kh, kl, k_pool.data_ptr(), ks[0], ks[1],
-            None if v is None else v.data_ptr(), vb, vh, vl, None if v is None else v_pool.data_ptr(), vs[0], vs[1],
-            B, H, L, pages, pos_p, new_p, (1 if rotate else 0) | (COMPRESS_BLOCK96 if shape[3] == RECORD96 else 0))
+    _launch(_COMPRESS_PAGED, dev, k.data_ptr(), kb, kh, kl, k_pool.data_ptr(), ks[0], ks[1],
+            0 if v is None else v.data_ptr(), vb, vh, vl, 0 if v is None else v_pool.data_ptr(), vs[0], vs[1],
+            B, H, L, *pages, pos_p, new_p, (1 if rotate else 0) | (COMPRESS_BLOCK96 if shape[3] == RECORD96 else 0))
 
 
 def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_table: torch.Tensor,
@@ -1037,9 +1045,9 @@ def dequantize_paged(k_pool: torch.Tensor, v_pool: torch.Tensor | None, block_ta
     elif len(out) != n or any(tuple(t.shape) != want or t.dtype is not torch.float16 or not t.is_contiguous()
                               or t.device != dev for t in out):
         raise RuntimeError("out must hold contiguous float16 tensors [B, Hkv, max_len, 128] on the pools' device")
-    _launch(_lib.ecc_dequantize_paged, "dequantize_paged", dev, k_pool.data_ptr(), ks[0], ks[1], out[0].data_ptr(),
-            None if n == 1 else v_pool.data_ptr(), vs[0], vs[1], None if n == 1 else out[1].data_ptr(), B, H,
-            int(max_len), pages, lens, (1 if unrotate else 0) | (2 if shape[3] == RECORD96 else 0))
+    _launch(_DEQUANTIZE_PAGED, dev, k_pool.data_ptr(), ks[0], ks[1], out[0].data_ptr(),
+            0 if n == 1 else v_pool.data_ptr(), vs[0], vs[1], 0 if n == 1 else out[1].data_ptr(), B, H,
+            int(max_len), *pages, lens, (1 if unrotate else 0) | (2 if shape[3] == RECORD96 else 0))
     return out if n == 2 else out[0]
 
 
@@ -1089,8 +1097,8 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     lens = _per_sequence(seq_lens, "seq_lens", dev, B)
     if window < 0 or sinks < 0 or (sinks and not window):
         raise RuntimeError("window and sinks must not be negative, and sinks need a window")
-    capacity = pages.width * pages.page_size
-    wp, wb, wh = (None, 0, 0) if weights is None else _weights_like(weights, "weights", B, hkv, capacity, dev)
+    capacity = pages[2] * pages[3]
+    wp, wb, wh = (0, 0, 0) if weights is None else _weights_like(weights, "weights", B, hkv, capacity, dev)
     if out is None:
         out = torch.empty_like(q3) if len(qs) == 4 else torch.empty((B, hq, 1, D), dtype=torch.float16, device=dev)
     elif not out.is_contiguous() or out.dtype is not torch.float16 or out.numel() != B * hq * D or out.device != dev:
@@ -1098,8 +1106,8 @@ def decode_attention_paged(query: torch.Tensor, k_pool: torch.Tensor, v_pool: to
     lse = torch.empty((B, hq), dtype=torch.float32, device=dev) if return_lse else None
     flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | (BLOCK96 if shape[3] == RECORD96 else 0)
     ws = _scratch(workspace, dev, _decode_paged_bytes(B, hq, hkv, capacity, weights is not None, dev.index))
-    _launch(_lib.ecc_decode_paged, "decode_attention_paged", dev, q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-            ks[0], ks[1], pages, lens, out.data_ptr(), None if lse is None else lse.data_ptr(), wp, wb, wh, ws.data_ptr(),
+    _launch(_DECODE_PAGED, dev, q3.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+            ks[0], ks[1], *pages, lens, out.data_ptr(), 0 if lse is None else lse.data_ptr(), wp, wb, wh, ws.data_ptr(),
             ws.numel() * ws.element_size(), B, hq, hkv, 0.0 if sm_scale is None else float(sm_scale),
             min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff), flags)
     return (out, lse) if return_lse else out
@@ -1138,11 +1146,11 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
     lens = _per_sequence(seq_lens, "seq_lens", dev, B)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise RuntimeError("budget must be positive and hold the sinks and the recent tokens")
-    if outs.width * outs.page_size < budget:
+    if outs[2] * outs[3] < budget:
         raise RuntimeError(f"out_table names fewer than {budget} tokens per sequence")
-    if outs.table == pages.table:
+    if outs[0] == pages[0]:
         raise RuntimeError("out_table must name other pages than block_table")
-    capacity = pages.width * pages.page_size
+    capacity = pages[2] * pages[3]
     wp, wb, wh = _weights_like(weights, "weights", B, hkv, capacity, dev, written=False)
     if out_weights is None:
         out_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
@@ -1160,8 +1168,8 @@ def evict_paged(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.T
             or kept.device != dev:
         raise RuntimeError("kept must be a contiguous int32 tensor [B, Hkv, budget] on the pools' device")
     ws = _scratch(workspace, dev, _evict_paged_bytes(shape[0]))
-    _launch(_lib.ecc_evict_paged, "evict_paged", dev, k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1], pages, lens,
-            wp, wb, wh, outs, op, ob, oh, out_weights.shape[2], kept.data_ptr(), B, hkv, int(budget), int(sinks),
+    _launch(_EVICT_PAGED, dev, k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1], *pages, lens,
+            wp, wb, wh, *outs, op, ob, oh, out_weights.shape[2], kept.data_ptr(), B, hkv, int(budget), int(sinks),
             int(recent), shape[3], ws.data_ptr(), ws.numel() * ws.element_size())
     return out_weights, kept
 
@@ -1173,7 +1181,7 @@ _SAMPLE_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 def _setting(v, name: str, dtype, B: int, device, lo: float, hi: float):
-    """(device pointer or None, value) of a sampling setting: one value for
+    """(device pointer or 0, value) of a sampling setting: one value for
     every row, or a [B] tensor on the GPU (whose values are not looked at)."""
     if isinstance(v, torch.Tensor):
         _require_cuda(v, name)
@@ -1182,7 +1190,7 @@ def _setting(v, name: str, dtype, B: int, device, lo: float, hi: float):
         return v.data_ptr(), 0
     if not lo <= v <= hi:
         raise RuntimeError(f"{name} must lie in [{lo}, {hi}], got {v}")
-    return None, v
+    return 0, v
 
 
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -1221,7 +1229,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     elif tuple(out.shape) != (B,) or out.dtype != torch.int64 or not out.is_contiguous() or out.device != dev:
         raise RuntimeError("out must be a contiguous int64 tensor [B] on the logits' device")
     logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprobs else None
-    _launch(_lib.ecc_sample, "sample_tokens", dev, logits.data_ptr(), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V,
+    _launch(_SAMPLE, dev, logits.data_ptr(), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V,
             uniform.data_ptr(), t[0], float(t[1]), k[0], int(k[1]), p[0], float(p[1]), m[0], float(m[1]), out.data_ptr(),
-            None if logprob is None else logprob.data_ptr())
+            0 if logprob is None else logprob.data_ptr())
     return (out, logprob) if return_logprobs else out

@@ -483,6 +483,19 @@ int ecc_sample(const void *logits, int64_t row_stride, int dtype, int B, int64_t
                float top_p_all, const float *min_p, float min_p_all, int64_t *token, float *logprob,
                ecc_stream_t stream);
 
+/* ---- arguments as words ----------------------------------------------------
+ * The call `entry` (ECC_CALL_*) with its arguments, in the order of its
+ * declaration above, as 64-bit words: pointers and integers as they are, floats
+ * as doubles, a page table in place as its five members.  For bindings that pay
+ * for every argument.  An integer that does not fit its type gives
+ * ECC_ERR_SHAPE. */
+#define ECC_CALL_COMPRESS_PAGED 0
+#define ECC_CALL_DEQUANTIZE_PAGED 1
+#define ECC_CALL_DECODE_PAGED 2
+#define ECC_CALL_EVICT_PAGED 3
+#define ECC_CALL_SAMPLE 4
+int ecc_call(int entry, const int64_t *words);
+
 #ifdef __cplusplus
 }
 #endif

@@ -178,3 +178,46 @@ def test_written_weights_must_not_overlap():
         with pytest.raises(RuntimeError, match="overlap"):
             look(t, t.shape[0], t.shape[1])
         look(t, t.shape[0], t.shape[1], written=False)  # to be read only
+
+
+def test_arguments_as_words(lib):
+    """ecc_call gives what the typed entry points give, up to the first device call."""
+    import struct
+    call = lib.ecc_call
+    call.argtypes = [ctypes.c_int, ctypes.c_void_p]
+    pg = (4096, 4, 4, 16, 10)
+
+    def words(layout, *v):
+        return struct.pack("=" + layout, *v)
+
+    def compress(x=4096, B=1, L=4, pages=pg, mode=1):
+        return call(0, words("26q", x, 0, 0, 128, 4096, 32, 16, 0, 0, 0, 128, 0, 32, 16, B, 1, L, *pages, 4096, 0, mode, 0))
+
+    def dequantize(x=4096, B=1, n=4, pages=pg, mode=0):
+        return call(1, words("19q", x, 32, 16, 4096, 0, 0, 0, 0, B, 1, n, *pages, 4096, mode, 0))
+
+    def decode(q=4096, B=1, hq=2, scale=0.0, sinks=0, flags=0, pages=pg, room=1 << 30):
+        return call(2, words("21qd4q", q, 4096, 4096, 32, 16, *pages, 4096, 4096, 0, 0, 0, 0, 4096, room, B, hq, 1, scale,
+                             0, sinks, flags, 0))
+
+    def evict(k=4096, B=1, budget=8, recent=0, rec=128, room=1 << 20, pages=pg):
+        return call(3, words("32q", k, 4096, 32, 16, *pages, 4096, 4096, 64, 64, 8192, *pages[1:], 4096, 64, 64, 64, 4096, B,
+                             1, budget, 0, recent, rec, 4096, room, 0))
+
+    def sample(x=4096, dtype=0, B=1, V=8, t0=1.0, k0=0, p0=1.0, m0=0.0):
+        return call(4, words("7qd3qdqd3q", x, 8, dtype, B, V, 4096, 0, t0, 0, k0, 0, p0, 0, m0, 4096, 0, 0))
+
+    assert compress(B=0) == OK and dequantize(B=0) == OK and decode(B=0) == OK and evict(B=0) == OK and sample(B=0) == OK
+    for got, code in ((compress(x=0), NULL), (compress(L=-1), SHAPE), (compress(mode=4), SHAPE), (compress(x=4104), ALIGN),
+                      (compress(B=1 << 32), SHAPE), (compress(pages=(4096, 4, 4, 24, 10)), SHAPE),
+                      (dequantize(x=0), NULL), (dequantize(n=-1), SHAPE), (dequantize(mode=4), SHAPE),
+                      (dequantize(x=4104), ALIGN), (dequantize(pages=(4098, 4, 4, 16, 10)), ALIGN),
+                      (decode(q=0), NULL), (decode(q=4104), ALIGN), (decode(hq=9), SHAPE), (decode(scale=float("nan")), PARAM),
+                      (decode(scale=float("inf")), PARAM), (decode(scale=1e300), PARAM), (decode(sinks=1), SHAPE),
+                      (decode(flags=64), SHAPE), (decode(hq=2 + (1 << 32)), SHAPE), (decode(pages=(0, 4, 4, 16, 10)), NULL),
+                      (evict(k=0), NULL), (evict(recent=9), SHAPE), (evict(rec=64), SHAPE), (evict(room=0), WORKSPACE),
+                      (evict(budget=8 - (1 << 32)), SHAPE),
+                      (sample(x=0), NULL), (sample(x=4097), ALIGN), (sample(dtype=3), SHAPE), (sample(V=0), SHAPE),
+                      (sample(t0=-1.0), PARAM), (sample(k0=-1), PARAM), (sample(k0=1 << 31), SHAPE), (sample(p0=0.0), PARAM),
+                      (sample(m0=1.5), PARAM), (call(5, words("q", 0)), SHAPE), (call(0, None), NULL)):
+        assert got == code
