@@ -1225,10 +1225,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     p = _setting(top_p, "top_p", torch.float32, B, dev, 2.0 ** -126, math.inf)
     m = _setting(min_p, "min_p", torch.float32, B, dev, 0.0, 1.0)
     if out is None:
-        out = torch.empty((B,), dtype=torch.int64, device=dev)
+        out = torch.empty_like(uniform, dtype=torch.int64)
     elif tuple(out.shape) != (B,) or out.dtype != torch.int64 or not out.is_contiguous() or out.device != dev:
         raise RuntimeError("out must be a contiguous int64 tensor [B] on the logits' device")
-    logprob = torch.empty((B,), dtype=torch.float32, device=dev) if return_logprobs else None
+    logprob = torch.empty_like(uniform) if return_logprobs else None
     _launch(_SAMPLE, dev, logits.data_ptr(), logits.stride(0), _SAMPLE_TYPES[logits.dtype], B, V,
             uniform.data_ptr(), t[0], float(t[1]), k[0], int(k[1]), p[0], float(p[1]), m[0], float(m[1]), out.data_ptr(),
             0 if logprob is None else logprob.data_ptr())
