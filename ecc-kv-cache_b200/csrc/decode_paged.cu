@@ -294,8 +294,9 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         uint4 qw[4];
         load_q(qw, cons.b, cons.h);
         start_run();
-        for (int s = 0; s < kStages && s < ntiles; ++s) issue_next(s, s + 1 < ntiles);
-        L.set_query(qw, (a.flags & ECC_DECODE_ROTATE_Q) != 0);
+        issue_next(0, ntiles > 1);
+        L.set_query(qw, (a.flags & ECC_DECODE_ROTATE_Q) != 0);  // while the first copies are issued
+        for (int s = 1; s < kStages && s < ntiles; ++s) issue_next(s, s + 1 < ntiles);
     }
     L.lane8 = (uint32_t)lane * 8u;
     L.lane_hi = lane_hi_of(lane);
