@@ -147,8 +147,12 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    for (int v = warp; v < 256; v += kWarps)
-        reinterpret_cast<uint2 *>(sm + kSmLut + v * 256)[lane] = lut_entry(s_cent, v, lane);
+    // a half-warp writes a row of the table, a lane the entries of two lanes (both of one half)
+#pragma unroll 4
+    for (int v = 2 * warp + (lane >> 4); v < 256; v += 2 * kWarps) {
+        const uint2 e = lut_entry(s_cent, v, 2 * (lane & 15));
+        reinterpret_cast<uint4 *>(sm + kSmLut + v * 256)[lane & 15] = make_uint4(e.x, e.y, e.x, e.y);
+    }
     pdl_trigger();
     pdl_wait();  // everything above touched shared memory only
 
