@@ -115,15 +115,14 @@ __global__ void __launch_bounds__(kReadWarps * 32, 2) dequant_paged_kernel(const
     // entry v, copy l (l = lane mod 16): (hi, lo) fp16x2 words of the codes v & 15, v >> 4, or their fp32 values, at
     // 256 v + 8 l: the offset is one byte permutation
     extern __shared__ __align__(16) uint8_t tab[];
-    for (int i = threadIdx.x; i < 256 * 16; i += blockDim.x) {
-        const int v = i >> 4;
-        uint2 *const to = reinterpret_cast<uint2 *>(tab + 256 * v) + (i & 15);
-        float lo = lm(0), hi = lm(0);
+    static_assert(kReadWarps * 32 == 256, "a thread has one low code, one copy and all high codes");
+    float lo = lm(0);
 #pragma unroll
-        for (int k = 1; k < 16; ++k) {
-            lo = (v & 15) == k ? lm(k) : lo;
-            hi = (v >> 4) == k ? lm(k) : hi;
-        }
+    for (int k = 1; k < 16; ++k) lo = (threadIdx.x >> 4) == k ? lm(k) : lo;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const float hi = lm(k);
+        uint2 *const to = reinterpret_cast<uint2 *>(tab + 256 * (16 * k + (threadIdx.x >> 4))) + (threadIdx.x & 15);
         if (kRotate) {
             const __half2 x = __floats2half2_rn(lo, hi);
             const __half2 y = __floats2half2_rn(lo - __low2float(x), hi - __high2float(x));
