@@ -24,7 +24,7 @@ constexpr int kWarps = 12;          // warps per CTA (384 threads)
 constexpr int kStages = 2;          // ring stages per warp
 constexpr int kTile = 32;           // tokens per stage (two 16-token MMA sub-tiles)
 constexpr int kStageBytes = 6144;
-constexpr int kOffKC = 0, kOffKS = 2048, kOffVC = 3072, kOffVS = 5120;  // 32 x 64 B, 32 x 32 B, ...
+constexpr int kOffKC = 0, kOffKS = kOffKC + 32 * 64, kOffVC = kOffKS + 32 * 32, kOffVS = kOffVC + 32 * 64;
 constexpr int kSubC = 1024, kSubS = 512;  // offset of sub-tile 1 in the code / syndrome boxes
 constexpr int kThreads = kWarps * 32;
 constexpr int kLutBytes = 65536;
