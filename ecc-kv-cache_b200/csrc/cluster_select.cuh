@@ -318,7 +318,8 @@ __device__ __forceinline__ uint32_t join_lists(const Cluster &cl, unsigned long 
 // largest power of two up to 8 with which all of them run at the same time and
 // every CTA has `least` elements.  A cluster lives inside one GPC, so fewer fit
 // than the SMs would hold (16 rows in clusters of 8: 21 us in two waves where
-// clusters of 4 take 14).  Asked once per device.
+// clusters of 4 take 14).  Asked once per device; kernels of one signature share
+// the answer (a CTA of kThreads with this much shared memory has an SM to itself).
 constexpr size_t kMostShared = 227 * 1024;
 template <typename... KArgs>
 static inline int cluster_size(void (*kernel)(KArgs...), int64_t clusters, int64_t n, int least) {
