@@ -377,8 +377,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         // x, and spread however the logits lie
         Bins &bins = *reinterpret_cast<Bins *>(sh.hist);
         unsigned long long *list = reinterpret_cast<unsigned long long *>(sh.hist);
-        const float inv_bin = fminf(64.0f / temp, 3e38f);
-        auto distance = [best, inv_bin](float x) { return (best - x) * inv_bin; };  // in bins; -inf: infinity or NaN
+        // (above 0 for an infinite temperature too: a logit of -inf is infinitely far, never NaN bins, which would
+        // pass every test for a bin; finite logits are at most 8 bins off then, in their order)
+        const float inv_bin = fmaxf(fminf(64.0f / temp, 3e38f), 1.2e-38f);
+        auto distance = [best, inv_bin](float x) { return (best - x) * inv_bin; };  // in bins; -inf: infinity
         auto bin_of = [distance](float x) {
             const float d = distance(x);
             return d < (float)(kBins - 1) ? (int)d : kBins - 1;

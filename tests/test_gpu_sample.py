@@ -161,6 +161,38 @@ def test_sample_extreme_temperatures(T, scale):
         check(x, u, T=T, **s)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V,allowed", [(9000, 100), (128256, 100), (128256, 4096), (128256, 5000), (60, 7)])
+def test_sample_infinite_temperature_over_a_masked_row(V, allowed, dtype):
+    """Every allowed token weighs the same, a masked one (-inf or NaN) nothing: with equal weights the kept tokens are
+    the first by (logit, index) and the draw is token floor(u * kept) of them, ascending."""
+    import custom_ecc_cuda as ops
+    rng = np.random.default_rng(V + allowed)
+    x = np.full((6, V), -np.inf, np.float32)
+    ids = [np.sort(rng.choice(V, allowed, replace=False)) for _ in range(6)]
+    for b in range(6):
+        x[b, rng.choice(V, V // 8, replace=False)] = np.nan
+        x[b, ids[b]] = rng.normal(size=allowed)
+    xs = torch.from_numpy(x).to(TYPES[dtype])
+    x = xs.float().numpy()
+    u = np.array([0.0, 0.2, 0.4999, 0.71, 0.93, 0.99999], np.float32)
+    inf = torch.full((6,), float("inf"), device="cuda")
+    for k, p in ((0, 1.0), (50, 1.0), (0, 0.35), (50, 0.55), (3000, 1.0), (3000, 0.35), (V - 1, 1.0)):
+        for T in (float("inf"), inf):
+            out = torch.full((6,), -7, device="cuda")
+            tok, lp = ops.sample_tokens(xs.cuda(), torch.from_numpy(u).cuda(), temperature=T, top_k=k, top_p=p,
+                                        return_logprobs=True, out=out)
+            for b in range(6):
+                order = ids[b][np.lexsort((ids[b], -x[b, ids[b]]))]
+                order = order[:k] if k else order
+                if p < 1:
+                    order = order[:int(np.ceil(np.float64(np.float32(p)) * len(order)))]
+                want = np.sort(order)[int(np.float64(u[b]) * len(order))]
+                assert int(tok[b]) == want, (k, p, b)
+                l = np.log(len(order))
+                assert abs(float(lp[b]) + l) <= 2.0 ** -24 * l + 2.0 ** -40
+
+
 def test_sample_distribution():
     """Evenly spaced numbers draw every token in proportion to its probability, to one part in their count."""
     import custom_ecc_cuda as ops
