@@ -665,10 +665,17 @@ static int make_map(CUtensorMap *m, const void *base, int64_t seq_len, int Hkv, 
     cuuint64_t strides[3] = {(cuuint64_t)rb, sh, sb};
     cuuint32_t box[4] = {box_x, (cuuint32_t)box_rows, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    const CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box,
-                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? ECC_OK : ECC_ERR_CUDA;
+    const auto encode = [&]() {
+        return g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (encode()) return ECC_OK;
+    // The first CUDA call of a host thread: the driver's call, unlike the runtime's, does not make the device's
+    // context current by itself.
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return ECC_ERR_CUDA;
+    return encode() ? ECC_OK : ECC_ERR_CUDA;
 }
 
 // The four maps of a launch: K codes (64-byte rows, no swizzle: the K code

@@ -259,6 +259,34 @@ def test_decode_from_two_threads_on_one_stream():
         assert len(outs[i]) == 200 and all(torch.equal(o, cases[i][1]) for o in outs[i])
 
 
+@pytest.mark.parametrize("which", ["paged", "contiguous", "masked", "device length"])
+def test_decode_as_the_first_call_of_a_thread(which):
+    """A thread that has made no CUDA call yet: no context is current in it."""
+    import threading
+    import custom_ecc_cuda as ops
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(2, 2, 2, 300, 128, generator=g, device="cuda").half()
+    kp = torch.zeros(2, 2, 300, 128, dtype=torch.uint8, device="cuda")
+    vp = torch.zeros_like(kp)
+    ops.compress_pair_into(x[0], x[1], kp, vp)
+    q = torch.randn(2, 8, 1, 128, generator=g, device="cuda").half()
+    table, n, start, one = torch.arange(2, dtype=torch.int32, device="cuda")[:, None], i32([300, 45]), i32([0, 99]), i32([300])
+    ws = torch.empty(16 << 20, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    call = {"paged": lambda: ops.decode_attention_paged(q, kp, vp, table, n, workspace=ws, out=out),
+            "contiguous": lambda: ops.decode_attention(q, kp, vp, 300, workspace=ws, out=out),
+            "masked": lambda: ops.decode_attention_masked(q, kp, vp, 300, start, workspace=ws, out=out),
+            "device length": lambda: ops.decode_attention_dev(q, kp, vp, one, workspace=ws, out=out)}[which]
+    want = call().clone()
+    out.zero_()
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=call)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
 # ------------------------------------------------------------------ append and read-back
 @pytest.mark.parametrize("L,hkv,ps,rec", [(1, 2, 16, 128), (17, 3, 32, 96), (40, 1, 48, 128), (700, 4, 64, 128),
                                           (700, 4, 64, 96)])
