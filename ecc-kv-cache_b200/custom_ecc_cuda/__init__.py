@@ -120,6 +120,10 @@ def _load():
 _lib = _load()
 _ws_lock = threading.Lock()
 _ws_cache: dict = {}
+# By device: held while a call's launches are issued, because they share a
+# workspace with other calls on the stream (_workspace, _scratch): those of
+# another thread on the same stream must not come between them.
+_launch_locks = tuple(threading.Lock() for _ in range(64))
 
 
 def _check(rc: int, what: str):
@@ -450,7 +454,7 @@ def decode_attention(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     flags |= _KERNEL_FLAGS[kernel] | _rec_flag(k_pool)
     scale = float(sm_scale) if sm_scale is not None else 0.0
     need = decode_workspace_size(B, hq, hkv, seq_len, num_splits)
-    with torch.cuda.device(q3.device):
+    with torch.cuda.device(q3.device), _launch_locks[q3.device.index & 63]:
         ws = workspace if workspace is not None else _workspace(q3.device, need)
         if ws.numel() < need:
             raise RuntimeError(f"workspace too small: {ws.numel()} < {need} bytes")
@@ -489,7 +493,7 @@ def decode_attention_masked(query: torch.Tensor, k_pool: torch.Tensor, v_pool: t
         raise RuntimeError("out must be a contiguous float16 tensor of B*Hq*128 elements")
     flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | _rec_flag(k_pool)
     need = decode_workspace_size(B, hq, hkv, seq_len, 0)
-    with torch.cuda.device(q3.device):
+    with torch.cuda.device(q3.device), _launch_locks[q3.device.index & 63]:
         ws = workspace if workspace is not None else _workspace(q3.device, need)
         if ws.numel() < need:
             raise RuntimeError(f"workspace too small: {ws.numel()} < {need} bytes")
@@ -819,7 +823,7 @@ def decode_attention_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torc
         out = torch.empty((B, hq, 1, D), dtype=torch.float16, device=q3.device)
     flags = (ROTATE_Q if rotate_q else 0) | (UNROTATE_OUT if unrotate_out else 0) | _rec_flag(k_pool)
     need = decode_dev_workspace_size(B, hq, hkv, cap)
-    with torch.cuda.device(q3.device):
+    with torch.cuda.device(q3.device), _launch_locks[q3.device.index & 63]:
         ws = workspace if workspace is not None else _workspace(q3.device, need)
         if ws.numel() < need:
             raise RuntimeError(f"workspace too small: {ws.numel()} < {need} bytes")
@@ -868,9 +872,6 @@ def decode_partials_dev(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 # ---------------------------------------------------------------------------
 # Paged cache: sequences of any lengths in pages of a shared pool
 # ---------------------------------------------------------------------------
-_launch_locks = tuple(threading.Lock() for _ in range(64))  # by device
-
-
 class _Entry:
     """An entry point of ecc_call: its number and the layout of its words (q:
     pointers and integers, d: floats; the stream comes last)."""
@@ -888,9 +889,7 @@ _SAMPLE = _Entry(4, "sample_tokens", "7qd3qdqd3q")
 
 def _launch(entry: _Entry, dev: torch.device, *args) -> None:
     """The entry point with these arguments and the current stream of dev, with
-    dev the current device.  One call at a time: the launches of a call share a
-    workspace, and those of another thread on the same stream must not come
-    between them."""
+    dev the current device, one call at a time (_launch_locks)."""
     i = dev.index
     try:
         words = entry.pack(*args, torch._C._cuda_getCurrentRawStream(i))

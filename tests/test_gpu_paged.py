@@ -287,6 +287,70 @@ def test_decode_as_the_first_call_of_a_thread(which):
     assert torch.equal(out, want)
 
 
+def test_calls_that_share_a_workspace_issue_their_launches_one_at_a_time(monkeypatch):
+    """The contiguous decodes take the workspace of the paged calls on their stream: every one of these entry points is
+    called with the device's lock held, so no launch of another thread comes between its launches."""
+    import custom_ecc_cuda as ops
+    real, seen = ops._lib, []
+
+    class Recording:
+        def __getattr__(self, name):
+            fn = getattr(real, name)
+            if name not in ("ecc_call", "ecc_decode", "ecc_decode_masked", "ecc_decode_dev"):
+                return fn
+
+            def call(*args):
+                seen.append((name, ops._launch_locks[0].locked()))
+                return fn(*args)
+            return call
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(2, 2, 2, 64, 128, generator=g, device="cuda").half()
+    kp = torch.zeros(2, 2, 64, 128, dtype=torch.uint8, device="cuda")
+    vp = torch.zeros_like(kp)
+    ops.compress_pair_into(x[0], x[1], kp, vp)
+    q = torch.randn(2, 8, 1, 128, generator=g, device="cuda").half()
+    table = torch.arange(2, dtype=torch.int32, device="cuda")[:, None]
+    monkeypatch.setattr(ops, "_lib", Recording())
+    outs = [ops.decode_attention(q, kp, vp, seq_len=60), ops.decode_attention_masked(q, kp, vp, 60, i32([0, 0])),
+            ops.decode_attention_dev(q, kp, vp, i32([60])), ops.decode_attention_paged(q, kp, vp, table, i32([60, 60]))]
+    assert seen == [("ecc_decode", True), ("ecc_decode_masked", True), ("ecc_decode_dev", True), ("ecc_call", True)]
+    assert not ops._launch_locks[0].locked()
+    for o in outs[1:]:
+        assert (o.float() - outs[0].float()).abs().max() <= 2.0 ** -10 * outs[0].float().abs().max()
+
+
+def test_contiguous_and_paged_decode_from_threads_on_one_stream():
+    import threading
+    import custom_ecc_cuda as ops
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(2, 3, 2, 4000, 128, generator=g, device="cuda").half()
+    kp = torch.zeros(3, 2, 4000, 128, dtype=torch.uint8, device="cuda")
+    vp = torch.zeros_like(kp)
+    ops.compress_pair_into(x[0], x[1], kp, vp)
+    q = torch.randn(3, 8, 1, 128, generator=g, device="cuda").half()
+    table, n, start = torch.arange(3, dtype=torch.int32, device="cuda")[:, None], i32([4000, 17, 900]), i32([0, 9, 700])
+    calls = [lambda: ops.decode_attention_paged(q, kp, vp, table, n), lambda: ops.decode_attention(q, kp, vp, 3900),
+             lambda: ops.decode_attention_masked(q, kp, vp, 3500, start),
+             lambda: ops.decode_attention_dev(q, kp, vp, n[:1])]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    outs = [[] for _ in calls]
+
+    def run(i):
+        for _ in range(100):
+            outs[i].append(calls[i]())
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert len(o) == 100 and all(torch.equal(a, w) for a in o)
+
+
 # ------------------------------------------------------------------ append and read-back
 @pytest.mark.parametrize("L,hkv,ps,rec", [(1, 2, 16, 128), (17, 3, 32, 96), (40, 1, 48, 128), (700, 4, 64, 128),
                                           (700, 4, 64, 96)])
