@@ -136,6 +136,18 @@ class PagedErrorCorrectedCache(_HFCache):
         self._upload([b for b, n in enumerate(need) if n])
         self._mask_checked = False
 
+    def _ungrow(self, before: Tuple[List[int], List[int], List[int], List[int]]) -> None:
+        """Takes back a _grow whose tokens were not written; before: (lengths, tokens seen, pages held, lengths before
+        the last step) as they were."""
+        held = before[2]
+        back = [b for b, p in enumerate(self._pages) if len(p) > held[b]]
+        for b in reversed(back):
+            self._free += reversed(self._pages[b][held[b]:])
+            del self._pages[b][held[b]:]
+        self._len, self._seen, self._old_len = before[0], before[1], before[3]
+        self._upload(back)
+        self._pos.copy_(torch.tensor(self._old_len, dtype=torch.int32))
+
     def release(self, slots: Optional[Sequence[int]] = None) -> None:
         """Ends the sequences of the slots (default: all) and frees their pages."""
         slots = range(self.batch_size) if slots is None else slots
@@ -167,21 +179,33 @@ class PagedErrorCorrectedCache(_HFCache):
         new = [L] * B if new_lens is None else [int(n) for n in new_lens]
         if len(new) != B or min(new) < 0 or max(new) > L:
             raise RuntimeError(f"new_lens must hold {B} counts from 0 to {L}")
-        if layer_idx == 0:
-            self._grow(new)
-            self._new = None if new_lens is None else torch.tensor(new, dtype=torch.int32).to(self._device)
-        elif [n + m for n, m in zip(self._old_len, new)] != self._len:
-            raise RuntimeError("every layer of a step must append what layer 0 appended")
         k16 = key_states if key_states.dtype == torch.float16 else key_states.to(torch.float16)
         v16 = value_states if value_states.dtype == torch.float16 else value_states.to(torch.float16)
+        if layer_idx == 0:
+            before = (self._len, self._seen, [len(p) for p in self._pages], self._old_len)
+            last_new = self._new
+            self._grow(new)
+            try:
+                self._new = None if new_lens is None else torch.tensor(new, dtype=torch.int32).to(self._device)
+                self._write(k16, v16, 0)
+            except Exception:  # refused states, say: the sequences stay as they were
+                self._new = last_new
+                self._ungrow(before)
+                raise
+        elif [n + m for n, m in zip(self._old_len, new)] != self._len:
+            raise RuntimeError("every layer of a step must append what layer 0 appended")
+        else:
+            self._write(k16, v16, layer_idx)
+        self._last_layer = layer_idx
+        self._layer_fill[layer_idx] = max(self._seen)
+
+    def _write(self, k16: torch.Tensor, v16: torch.Tensor, layer_idx: int) -> None:
         kp, vp = self.layer_pools(layer_idx)
         if self.rotate_values:
             ops.compress_pair_paged(k16, v16, kp, vp, self.block_table, self._pos, new_lens=self._new)
         else:
             ops.compress_pair_paged(k16, None, kp, None, self.block_table, self._pos, new_lens=self._new)
             ops.compress_pair_paged(v16, None, vp, None, self.block_table, self._pos, new_lens=self._new, rotate=False)
-        self._last_layer = layer_idx
-        self._layer_fill[layer_idx] = max(self._seen)
 
     def context(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """The layer's K and V read back in the model's basis, [B, Hkv, longest

@@ -148,6 +148,44 @@ def test_cache_refusals(cuda_device):
         cache.decode_attention(q, 0, attn_mask=mask)
 
 
+@pytest.mark.parametrize("rotate", [True, False])
+def test_refused_append_leaves_the_cache_as_it_was(cuda_device, rotate):
+    """Layer 0's states are refused by the operator (no contiguous rows, a base off 16 bytes, another device): lengths,
+    pages and positions stay, and the next append goes where it would have gone."""
+    from custom_kv import PagedErrorCorrectedCache
+    caches = [PagedErrorCorrectedCache(config(2), batch_size=2, max_cache_len=96, num_pages=9, page_size=16,
+                                       rotate_values=rotate) for _ in range(2)]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    first, second = states(caches[0], 2, 20, g), states(caches[0], 2, 30, g)
+
+    def look(c):
+        return (c.lengths, c.free_pages, c.seq_lens.tolist(), c.block_table.tolist(), c._pos.tolist(), c.get_seq_length(),
+                [list(p) for p in c._pages], list(c._free), list(c._seen))
+
+    for i, cache in enumerate(caches):
+        for step, (new, kv) in enumerate((([20, 7], first), ([9, 30], second))):
+            if i == 0:
+                k, v = kv[0]
+                flat = torch.zeros(k.numel() + 1, dtype=torch.float16, device="cuda")
+                off = flat[1:].view(k.shape)
+                turned = torch.empty(*k.shape[:2], 128, k.shape[2], dtype=torch.float16, device="cuda").transpose(2, 3)
+                was = look(cache)
+                for bad in ((off, v), (k, off), (turned, v), (k, turned), (k.cpu(), v), (k, v.cpu())):
+                    with pytest.raises(RuntimeError):
+                        cache.append(*bad, 0, new_lens=new)
+                    assert look(cache) == was
+            for layer, (k, v) in enumerate(kv):
+                cache.append(k, v, layer, new_lens=new)
+                if i == 0 and step == 1 and layer == 0:  # a refusal of a later layer can be mended by a second call
+                    with pytest.raises(RuntimeError):
+                        cache.append(k.cpu(), v.cpu(), 1, new_lens=new)
+    assert look(caches[0]) == look(caches[1])
+    assert caches[0].lengths == [29, 37]
+    for layer in range(2):
+        for x, y in zip(caches[0].context(layer), caches[1].context(layer)):
+            assert torch.equal(x, y)
+
+
 def _tiny_llama(seed=0, layers=2):
     from transformers import LlamaConfig, LlamaForCausalLM
     torch.manual_seed(seed)
