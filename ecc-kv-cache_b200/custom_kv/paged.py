@@ -255,14 +255,23 @@ class PagedErrorCorrectedCache(_HFCache):
         for i in range(0, len(slots), at_once):
             part = slots[i:i + at_once]
             fresh = [[self._free.pop() for _ in range(per)] for _ in part]
-            rows = torch.tensor(part, device=self._device)
-            table, lens = self.block_table[rows], self.seq_lens[rows]
-            out_table = torch.tensor(fresh, dtype=torch.int32).to(self._device)
-            for layer in range(self._num_layers):
-                kp, vp = self.layer_pools(layer)
-                w, _ = ops.evict_paged(kp, vp, table, lens, self.weights[layer][rows], out_table, budget, sinks=sinks,
-                                       recent=recent)
-                self.weights[layer][rows] = w
+            try:
+                rows = torch.tensor(part, device=self._device)
+                table, lens = self.block_table[rows], self.seq_lens[rows]
+                out_table = torch.tensor(fresh, dtype=torch.int32).to(self._device)
+                weights = []  # of the kept tokens: they count once every layer is cut
+                for layer in range(self._num_layers):
+                    kp, vp = self.layer_pools(layer)
+                    w, _ = ops.evict_paged(kp, vp, table, lens, self.weights[layer][rows], out_table, budget, sinks=sinks,
+                                           recent=recent)
+                    weights.append(w[:, :, :budget].clone())
+                    del w
+            except Exception:  # out of memory, say: the blocks were copied, nothing of the cache has changed
+                self._free += [p for pages in reversed(fresh) for p in reversed(pages)]
+                raise
+            for layer, w in enumerate(weights):
+                self.weights[layer, rows, :, :budget] = w
+                self.weights[layer, rows, :, budget:] = 0
             for b, pages in zip(part, fresh):
                 self._free += reversed(self._pages[b])
                 self._pages[b], self._len[b] = pages, budget

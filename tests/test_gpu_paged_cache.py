@@ -186,6 +186,47 @@ def test_refused_append_leaves_the_cache_as_it_was(cuda_device, rotate):
             assert torch.equal(x, y)
 
 
+def test_failed_eviction_leaves_the_cache_as_it_was(cuda_device, monkeypatch):
+    """An error in the second layer's cut (no memory for its results, say): pages, lengths, weights and blocks of every
+    layer stay, and the eviction can be asked for again."""
+    import custom_ecc_cuda as ops
+    from custom_kv import PagedErrorCorrectedCache
+    cache = PagedErrorCorrectedCache(config(3), batch_size=2, max_cache_len=64, num_pages=11, page_size=16,
+                                     collect_weights=True)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    for layer, (k, v) in enumerate(states(cache, 2, 60, g)):
+        cache.append(k, v, layer)
+    cache.weights.copy_(torch.rand(cache.weights.shape, generator=g, device="cuda"))
+    was = (cache.lengths, list(cache._free), cache.seq_lens.tolist(), cache.block_table.tolist())
+    weights, context = cache.weights.clone(), [cache.context(i) for i in range(3)]
+    real, calls = ops.evict_paged, []
+
+    def failing(*args, **kw):
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("no memory")
+        return real(*args, **kw)
+
+    monkeypatch.setattr(ops, "evict_paged", failing)
+    with pytest.raises(RuntimeError, match="no memory"):
+        cache.evict(30, sinks=2, recent=5)
+    assert (cache.lengths, list(cache._free), cache.seq_lens.tolist(), cache.block_table.tolist()) == was
+    assert torch.equal(cache.weights, weights)
+    for i in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(cache.context(i), context[i]))
+    assert cache.evict(30, sinks=2, recent=5) == [0, 1] and cache.lengths == [30, 30]
+    for i in range(3):
+        for b in range(2):
+            for h in range(2):
+                row = weights[i, b, h].cpu().numpy()
+                mid = sorted(range(2, 55), key=lambda t: (-row[t], t))[:23]
+                ids = list(range(2)) + sorted(mid) + list(range(55, 60))
+                assert np.array_equal(cache.weights[i, b, h, :30].cpu().numpy(), row[ids])
+                assert not cache.weights[i, b, h, 30:].any()
+                for x, y in zip(cache.context(i), context[i]):
+                    assert torch.equal(x[b, h], y[b, h, ids])
+
+
 def _tiny_llama(seed=0, layers=2):
     from transformers import LlamaConfig, LlamaForCausalLM
     torch.manual_seed(seed)
