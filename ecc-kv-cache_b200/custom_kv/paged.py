@@ -93,7 +93,6 @@ class PagedErrorCorrectedCache(_HFCache):
         self._layer_fill: List[int] = [0] * self._num_layers
         self._old_len: List[int] = [0] * self.batch_size
         self._new: Optional[torch.Tensor] = None
-        self._mask_checked = False
 
     # ------------------------------------------------------------------ #
     # pages                                                               #
@@ -134,7 +133,6 @@ class PagedErrorCorrectedCache(_HFCache):
         self._len = want
         self._seen = [n + m for n, m in zip(self._seen, new)]
         self._upload([b for b, n in enumerate(need) if n])
-        self._mask_checked = False
 
     def _ungrow(self, before: Tuple[List[int], List[int], List[int], List[int]]) -> None:
         """Takes back a _grow whose tokens were not written; before: (lengths, tokens seen, pages held, lengths before
@@ -221,12 +219,12 @@ class PagedErrorCorrectedCache(_HFCache):
                          attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One decode step of attention of ``query`` [B, Hq, 1, 128] over every
         slot's own sequence (the new token already appended).  ``attn_mask`` may
-        hide nothing (looked at once per step): sequences hold no padding."""
-        if attn_mask is not None and not self._mask_checked:
+        hide nothing (every layer's is looked at, which waits for the GPU): sequences
+        hold no padding."""
+        if attn_mask is not None:
             see = attn_mask if attn_mask.dtype == torch.bool else attn_mask > torch.finfo(attn_mask.dtype).min / 2
             if not bool(see.all()):
                 raise RuntimeError("PagedErrorCorrectedCache holds no padding: the attention mask hides cached tokens")
-            self._mask_checked = True
         kp, vp = self.layer_pools(layer_idx)
         q16 = query if query.dtype == torch.float16 else query.to(torch.float16)
         out = ops.decode_attention_paged(q16, kp, vp, self.block_table, self.seq_lens, sm_scale=sm_scale,

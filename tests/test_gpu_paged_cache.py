@@ -227,6 +227,24 @@ def test_failed_eviction_leaves_the_cache_as_it_was(cuda_device, monkeypatch):
                     assert torch.equal(x[b, h], y[b, h, ids])
 
 
+def test_every_layers_mask_is_looked_at(cuda_device):
+    """A model's layers may have masks of their own (a sliding window in every other one)."""
+    from custom_kv import PagedErrorCorrectedCache
+    cache = PagedErrorCorrectedCache(config(3), batch_size=2, max_cache_len=64, page_size=16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for layer, (k, v) in enumerate(states(cache, 2, 40, g)):
+        cache.append(k, v, layer)
+    q = torch.randn(2, 4, 1, 128, generator=g, device="cuda").half()
+    whole = torch.ones(2, 1, 1, 40, dtype=torch.bool, device="cuda")
+    part = whole.clone()
+    part[..., :8] = False
+    for layer in range(3):
+        assert torch.equal(cache.decode_attention(q, layer, attn_mask=whole), cache.decode_attention(q, layer))
+        for mask in (part, torch.zeros(2, 1, 1, 40, device="cuda").masked_fill(~part, torch.finfo(torch.float32).min)):
+            with pytest.raises(RuntimeError, match="padding"):
+                cache.decode_attention(q, layer, attn_mask=mask)
+
+
 def _tiny_llama(seed=0, layers=2):
     from transformers import LlamaConfig, LlamaForCausalLM
     torch.manual_seed(seed)
