@@ -219,12 +219,13 @@ class PagedErrorCorrectedCache(_HFCache):
                          attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One decode step of attention of ``query`` [B, Hq, 1, 128] over every
         slot's own sequence (the new token already appended).  ``attn_mask`` may
-        hide nothing (every layer's is looked at, which waits for the GPU): sequences
-        hold no padding."""
+        hide nothing and add nothing (every layer's is looked at, which waits for
+        the GPU): sequences hold no padding, and the kernel adds no bias."""
         if attn_mask is not None:
-            see = attn_mask if attn_mask.dtype == torch.bool else attn_mask > torch.finfo(attn_mask.dtype).min / 2
+            see = attn_mask if attn_mask.dtype == torch.bool else attn_mask == 0
             if not bool(see.all()):
-                raise RuntimeError("PagedErrorCorrectedCache holds no padding: the attention mask hides cached tokens")
+                raise RuntimeError("PagedErrorCorrectedCache holds no padding and adds no bias: the attention mask hides cached "
+                                   "tokens or adds to their scores")
         kp, vp = self.layer_pools(layer_idx)
         q16 = query if query.dtype == torch.float16 else query.to(torch.float16)
         out = ops.decode_attention_paged(q16, kp, vp, self.block_table, self.seq_lens, sm_scale=sm_scale,

@@ -245,6 +245,24 @@ def test_every_layers_mask_is_looked_at(cuda_device):
                 cache.decode_attention(q, layer, attn_mask=mask)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("value", [-1e4, -0.5, 1e-3, float("nan")])
+def test_masks_that_add_to_the_scores_are_refused(cuda_device, dtype, value):
+    """A finite stand-in for minus infinity, or a position bias: neither is dropped silently."""
+    from custom_kv import PagedErrorCorrectedCache
+    cache = PagedErrorCorrectedCache(config(1), batch_size=2, max_cache_len=64, page_size=16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    (k, v), = states(cache, 2, 40, g)
+    cache.append(k, v, 0)
+    q = torch.randn(2, 4, 1, 128, generator=g, device="cuda").half()
+    mask = torch.zeros(2, 1, 1, 40, dtype=dtype, device="cuda")
+    mask[1, ..., 0] = -0.0
+    assert torch.equal(cache.decode_attention(q, 0, attn_mask=mask), cache.decode_attention(q, 0))
+    mask[1, ..., 3] = value
+    with pytest.raises(RuntimeError, match="padding"):
+        cache.decode_attention(q, 0, attn_mask=mask)
+
+
 def _tiny_llama(seed=0, layers=2):
     from transformers import LlamaConfig, LlamaForCausalLM
     torch.manual_seed(seed)
