@@ -33,6 +33,8 @@ class PagedErrorCorrectedCache(_HFCache):
 
     Sequences hold no padding: a batch is appended at the end of every slot's
     own sequence, and an attention mask that hides cached tokens is refused.
+    A model takes one position for all slots unless it is told otherwise: with
+    slots of different lengths pass ``position_ids=cache.position_ids()``.
     ``get_seq_length`` counts the tokens seen (positions go on after an
     eviction); ``lengths`` are the tokens held."""
 
@@ -101,6 +103,29 @@ class PagedErrorCorrectedCache(_HFCache):
     def lengths(self) -> List[int]:
         """Tokens held per slot."""
         return list(self._len)
+
+    def position_ids(self) -> torch.Tensor:
+        """The position of every slot's next token, [B, 1] int64 on the GPU."""
+        return torch.tensor(self._seen, dtype=torch.int64).to(self._device)[:, None]
+
+    def check_positions(self, position_ids: Optional[torch.Tensor], position_embeddings=None) -> None:
+        """Refuses a model's step that rotates slots of different lengths all at one
+        position (what a model does by itself: the longest slot's).  Called
+        before the first layer with what its attention module is given; with
+        slots of different lengths it waits for the GPU."""
+        if min(self._seen) == max(self._seen):
+            return
+        if position_ids is not None:  # [.., B or 1, L]
+            per_slot = position_ids.dim() > 1 and position_ids.shape[-2] == self.batch_size
+            one = not per_slot or bool((position_ids[..., -1] == max(self._seen)).all())
+        elif position_embeddings is not None:  # (cos, sin), [B or 1, L, ..]
+            last = position_embeddings[1][:, -1]
+            one = last.shape[0] != self.batch_size or bool((last == last[:1]).all())
+        else:
+            return  # a model that does not show its positions
+        if one:
+            raise RuntimeError("the slots have different lengths, and the step's positions are the same for all of them: pass "
+                               "position_ids=cache.position_ids()")
 
     @property
     def free_pages(self) -> int:
@@ -286,7 +311,8 @@ class PagedErrorCorrectedCache(_HFCache):
         they are the whole context or a single token (the patched SDPA then
         reads the pages), otherwise the context read back, with the new states
         in the place of their reconstruction (all slots at one length,
-        nothing evicted: the model's causal mask counts the tokens seen)."""
+        nothing evicted: the model's causal mask counts the tokens seen).  The
+        states come rotated: slots of different lengths each at its own position."""
         L = key_states.shape[2]
         if L > 1 and layer_idx == 0 and (min(self._len) != max(self._len) or self._seen != self._len):
             raise RuntimeError("a chunk of several tokens needs all slots at one length and nothing evicted (append and "

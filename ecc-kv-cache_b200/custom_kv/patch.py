@@ -19,7 +19,8 @@ cache's last updated layer is the layer of the call.  For callers that reach
 SDPA without an ``update``, attention modules that carry a ``layer_idx``
 attribute (all transformers attention classes do) report their index through a
 forward pre-hook; the router uses that hint when the cache has no context for
-its last layer.
+its last layer.  A cache whose slots may have different lengths is shown the
+positions of the step by the same hook, before its first layer.
 
 The patch is process-global (torch's SDPA symbol) and not thread-safe, as in
 the reference.
@@ -54,7 +55,7 @@ class _DecodeRouter:
         self.saved_sdpa = F.scaled_dot_product_attention
         F.scaled_dot_product_attention = self.sdpa
         for module in _attention_modules(model):
-            self.hooks.append(module.register_forward_pre_hook(self._note_layer))
+            self.hooks.append(module.register_forward_pre_hook(self._note_layer, with_kwargs=True))
 
     def remove(self) -> None:
         if self.saved_sdpa is not None:
@@ -65,8 +66,12 @@ class _DecodeRouter:
         while self.hooks:
             self.hooks.pop().remove()
 
-    def _note_layer(self, module, args) -> None:
+    def _note_layer(self, module, args, kwargs) -> None:
         self.layer_hint = int(module.layer_idx)
+        check = getattr(self.cache, "check_positions", None)
+        used = kwargs.get("past_key_values", kwargs.get("past_key_value"))
+        if check is not None and self.layer_hint == 0 and used is self.cache:
+            check(kwargs.get("position_ids"), kwargs.get("position_embeddings"))
 
     def _layer_of_call(self) -> int:
         cache = self.cache

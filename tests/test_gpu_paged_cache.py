@@ -305,6 +305,65 @@ def test_model_runs_on_the_paged_cache(cuda_device):
             assert float(cache.weights.sum()) <= 6 * 2 * 2 * 4 * (1 + 1e-4)
 
 
+def test_slots_of_different_lengths_have_positions_of_their_own(cuda_device):
+    """A step whose positions are one for all slots is refused and leaves the cache as it was; with the cache's position_ids
+    the first layer's keys are, block for block, those of the same tokens in slots of one length."""
+    from custom_kv import paged_ecc_cache
+    model = _tiny_llama(2)
+    g = torch.Generator().manual_seed(9)
+    ids, toks = torch.randint(0, 1000, (2, 50), generator=g).cuda(), torch.randint(0, 1000, (3, 2, 1), generator=g).cuda()
+
+    def block(cache, slot, t):  # the key of token t in the first layer
+        return cache.layer_pools(0)[0][int(cache.block_table[slot, t // 16]), :, t % 16].clone()
+
+    new = dict(batch_size=2, max_cache_len=96, page_size=16)
+    with torch.no_grad():
+        alone = model(ids, use_cache=False).logits
+        with paged_ecc_cache(model, **new) as cache:  # slot 0 goes on at 50, as both slots do here
+            model(ids, past_key_values=cache, use_cache=True)
+            long = []
+            for i in range(3):
+                assert cache.position_ids().tolist() == [[50 + i], [50 + i]]
+                model(toks[i], past_key_values=cache, use_cache=True)
+                long.append(block(cache, 0, 50 + i))
+        with paged_ecc_cache(model, **new) as cache:  # slot 1 begins at 0
+            short = []
+            for i in range(3):
+                model(toks[i], past_key_values=cache, use_cache=True)
+                short.append(block(cache, 1, i))
+        with paged_ecc_cache(model, **new) as cache:
+            model(ids, past_key_values=cache, use_cache=True)
+            cache.release([1])
+            for i in range(3):
+                n = 50 + i
+                for bad in (dict(), dict(position_ids=torch.tensor([[n]], device="cuda")),
+                            dict(position_ids=torch.tensor([[n], [n]], device="cuda"))):
+                    with pytest.raises(RuntimeError, match="position_ids"):
+                        model(toks[i], past_key_values=cache, use_cache=True, **bad)
+                    assert cache.lengths == [n, i]
+                assert cache.position_ids().tolist() == [[n], [i]]
+                model(toks[i], past_key_values=cache, use_cache=True, position_ids=cache.position_ids())
+                assert torch.equal(block(cache, 0, n), long[i]) and torch.equal(block(cache, 1, i), short[i])
+            assert torch.equal(model(ids, use_cache=False).logits, alone)  # a pass without the cache is no concern of it
+
+
+def test_positions_a_model_shows_only_as_angles(cuda_device):
+    from custom_kv import PagedErrorCorrectedCache
+    cache = PagedErrorCorrectedCache(config(1), batch_size=2, max_cache_len=64, page_size=16)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    (k, v), = states(cache, 2, 40, g)
+    angles = torch.rand(2, 1, 128, generator=g, device="cuda")
+    same = angles[:1].expand(2, 1, 128)
+    for bad in (same, angles[:1]):
+        cache.check_positions(None, (bad.cos(), bad.sin()))  # slots of one length
+    cache.append(k, v, 0, new_lens=[40, 9])
+    cache.check_positions(None, (angles.cos(), angles.sin()))
+    cache.check_positions(None)
+    for bad in (same, angles[:1]):
+        with pytest.raises(RuntimeError, match="position_ids"):
+            cache.check_positions(None, (bad.cos(), bad.sin()))
+
+
 def test_recorded_settings_outlive_the_sampler(cuda_device):
     import custom_ecc_cuda as ops
     from custom_kv import Sampler, ecc_cache
