@@ -22,11 +22,11 @@
 // suffice for every distribution of lengths.  paged_merge_kernel joins them.
 //
 // Measured at 8 sequences x 65531 tokens, 32 query and 8 kv heads, pages of 128
-// tokens (1.07 GB of blocks): 223 us with the merge, 4.8 TB/s; the loads alone
-// take 169 us and the arithmetic alone 212.  It is bound by the latency of
-// dependent instructions at three warps of 168 registers per scheduler (ncu:
-// issue 56 %, shared-memory wavefronts 60 %, ALU 50 %, tensor 36 %), and in runs
-// of seconds by the 1000 W power cap (250 us at 1.70 GHz).
+// tokens (1.07 GB of blocks): 229 us with the merge, 4.7 TB/s; the loads alone
+// take 169 us.  It is bound by the latency of dependent instructions at three
+// warps of 168 registers per scheduler (ncu: issue 56 %, shared-memory
+// wavefronts 60 %, ALU 50 %, tensor 36 %), and in runs of seconds by the 1000 W
+// power cap.
 #include <algorithm>
 
 #include "decode_tile.cuh"
@@ -331,6 +331,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             L.lrun[e] = 0.0f;
             L.zrun[e] = 0.0f;
         }
+        L.vexp = 1;
         // ---------------- tiles of the segment ----------------
         for (int k = 0; k < seg_tiles; ++k) {
             bool ready = ok;
@@ -380,6 +381,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
             }
         }
         const int64_t slot = wid + row;
+        const float down = L.v_down();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float sg[4] = {0.f, 0.f, 0.f, 0.f};  // sign terms in the split columns (see decode_tma_kernel)
@@ -394,7 +396,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
                 const int h = 2 * L.c + e;
                 if (h >= G) continue;
                 float2 *pod = reinterpret_cast<float2 *>(a.po + (slot * G + h) * kD + d0);
-                *pod = make_float2(L.o[i][e] + (sg[e] + L.zrun[e]), L.o[i][2 + e] + (sg[2 + e] + L.zrun[e]));
+                *pod = make_float2(fmaf(L.o[i][e] + sg[e], down, L.zrun[e]), fmaf(L.o[i][2 + e] + sg[2 + e], down, L.zrun[e]));
             }
         }
         if (L.g == 0) {

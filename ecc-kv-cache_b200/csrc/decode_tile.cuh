@@ -263,6 +263,9 @@ struct Lane {
     float scale_log2;   // of the scores, with the query's scaling
     float scale_log2_0;  // kFine: without it
     uint32_t lane8, lane_hi;  // kFine: offsets in the paired table
+    int vexp;  // kFine: exponent field of the largest V scale or 2 alpha so far, 1..31 (see tile)
+    __device__ __forceinline__ float v_up() const { return kFine ? __int_as_float((127 + 29 - vexp) << 23) : 1.0f; }
+    __device__ __forceinline__ float v_down() const { return kFine ? __int_as_float((127 - 29 + vexp) << 23) : 1.0f; }
 
     // Query fragments of a row segment from the lane's fp16 query words qw
     // (dims 32c..32c+31 of its head): the centroid operand qc, the sign
@@ -487,8 +490,16 @@ struct Lane {
     // Per code byte i of the lane (dims 16g + 2i, 16g + 2i + 1 in rows g,
     // g + 8 of accumulator i), four products: centroids hi x ws, centroids
     // lo x ws, centroids hi x residual, signs x sign weights.
+    //
+    // kFine: all weights are times v_up() = 2^k, with which the largest V scale
+    // or 2 alpha met so far lies in [2^14, 2^15); the accumulators carry the
+    // factor, tile() rescales them when k falls and the segment's end takes it
+    // off.  fp16 and its residual end at 2^-25 absolute, so a weight is known to
+    // 2^-22 relative or 2^-39 of (the largest probability x the largest scale),
+    // where without the factor a token e^-12 below the largest with a scale of
+    // 0.05 had two bits.
     __device__ __forceinline__ void pv(const VRaw &v, const float (&p)[4]) {
-        constexpr float kUnit = kFine ? 1.0f / kCentScale : 1.0f;
+        const float up = v_up(), kUnit = kFine ? 1.0f / kCentScale * up : 1.0f;
         const float v_sa = h_lo(v.vma.x) * kUnit, v_aa = h_lo(v.vma.y);
         const float v_sb = h_lo(v.vmb.x) * kUnit, v_ab = h_lo(v.vmb.y);
         constexpr bool kSplitCols = G <= 4;
@@ -496,7 +507,7 @@ struct Lane {
         uint32_t mw[2], mr[2], ma[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const float sc = t ? v_sb : v_sa, al = (kSplitCols ? 2.0f : 1.0f) * (t ? v_ab : v_aa);
+            const float sc = t ? v_sb : v_sa, al = (kSplitCols ? 2.0f : 1.0f) * up * (t ? v_ab : v_aa);
             const float w0 = p[2 * t] * sc, w1 = p[2 * t + 1] * sc;
             mw[t] = pack_h2(w0, w1);
             mr[t] = pack_h2(w0 - h_lo(mw[t]), w1 - h_hi(mw[t]));
@@ -572,6 +583,13 @@ struct Lane {
     // `scores` is handed the log2-scaled scores of the two sub-tiles.
     template <class See, class Scores = NoScores>
     __device__ __forceinline__ void tile(uint32_t st, See see, Scores scores = Scores()) {
+        // kFine: the exponent field of the stage's largest V scale or 2 alpha, lane = token.  Asked for first (8 x 64k: 229
+        // us; behind the scores, where it is needed, 235; without it 222)
+        uint32_t top = 0;
+        if constexpr (kFine) {
+            const uint2 vm = lds64(st + kOffVS + 128 * g + 32 * c + (16 ^ (16 * (g & 1))));
+            top = __reduce_max_sync(0xffffffffu, max(vm.x & 0x7fffu, (vm.y & 0x7fffu) + 0x400u));
+        }
         const VRaw v0 = load_v(st + kOffVC, st + kOffVS);
         float s0[4], s1[4];
         qk(st + kOffKC, st + kOffKS, see, s0);
@@ -592,6 +610,14 @@ struct Lane {
             corr[e] = ex2(mrun[e] - mb[e]);
             mrun[e] = mnew;
         }
+        float corr_o[2] = {corr[0], corr[1]};
+        if constexpr (kFine) {
+            const int grown = max(vexp, (int)(top >> 10));
+            const float f = __int_as_float((127 + vexp - grown) << 23);
+            vexp = grown;
+            corr_o[0] *= f;
+            corr_o[1] *= f;
+        }
         float p0[4], p1[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -604,10 +630,10 @@ struct Lane {
         // the stage, so the compiler schedules the whole stage as one block
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            o[i][0] *= corr[0];
-            o[i][1] *= corr[1];
-            o[i][2] *= corr[0];
-            o[i][3] *= corr[1];
+            o[i][0] *= corr_o[0];
+            o[i][1] *= corr_o[1];
+            o[i][2] *= corr_o[0];
+            o[i][3] *= corr_o[1];
         }
         const VRaw v1 = load_v(st + kOffVC + kSubC, st + kOffVS + kSubS);
         {

@@ -79,6 +79,57 @@ def test_decode_batch_shapes(lens):
     check_decode(lens, 4, 2, 64, 128, rotate=True, seed=len(lens))
 
 
+def peaked(n, at, nats, v_scale, sink_v, g, rec, ps, seed):
+    """One kv head, n tokens of small keys and one, at `at`, that all heads' scores put `nats` above them; values of scale
+    `v_scale` (a number or a function of the token), that token's `sink_v`.  Returns q, pools and table."""
+    rng = np.random.default_rng(seed)
+    kp, vp, table = R.make_pools([n], ps, 1, rec, rng)
+    base = rng.normal(size=128)
+    q = (base * rng.uniform(0.97, 1.03, (1, g, 1)) + 0.01 * rng.normal(size=(1, g, 128))).astype(np.float16)
+
+    def metas(pool, scale):
+        for t in range(n):
+            m = np.array([scale[t], 0.0, 0.11 * scale[t]], np.float16)
+            pool[table[0, t // ps], 0, t % ps, 80:86] = m.view(np.uint8)
+
+    ks, vs = np.full(n, 0.05), np.array([v_scale(t) if callable(v_scale) else v_scale for t in range(n)], float)
+    if nats:
+        codes = np.where(q[0, 0] > 0, 14, 0).astype(np.uint8)  # the levels 2.4008 and -2.4008
+        kp[table[0, at // ps], 0, at % ps, :64] = codes[0::2] | (codes[1::2] << 4)
+        ks[at] = nats / (2.4008 * np.abs(q[0, 0].astype(float)).sum() * R.SM)
+        vs[at] = sink_v
+    metas(kp, ks)
+    metas(vp, vs)
+    return q, kp, vp, table
+
+
+@pytest.mark.parametrize("g,rec", [(4, 128), (8, 128), (1, 96)])
+@pytest.mark.parametrize("at,nats,v_scale,sink_v", [
+    (0, 12, 0.2, 1e-6), (0, 12, 0.05, 0.0), (0, 12, 0.02, 1e-6), (4095, 12, 0.05, 1e-6), (1777, 14, 0.5, 1e-6), (0, 17, 8.0, 1e-4),
+    (5, 8, 0.1, 1e-3), (0, 6, 1e-3, 1e-6), (0, 12, 0.05, 3.0), (0, 0, 1e-3, 0.0), (0, 0, lambda t: 10.0 ** (t % 47 / 9 - 3.5), 0.0),
+    (0, 10, lambda t: 10.0 ** (t / 1024 - 3), 1e-6), (0, 10, lambda t: 10.0 ** (1 - t / 1024), 1e-6), (0, 0, 2e4, 0.0)],
+    ids=lambda v: getattr(v, "__name__", str(v)))
+def test_decode_small_values_beside_a_dominating_token(at, nats, v_scale, sink_v, g, rec):
+    """Attention sinks with next to no value of their own: the output is made of probabilities far below the largest.
+    Sequences share one context, so many that a warp takes thousands of tokens in one piece.
+
+    The bound is attend()'s.  Its absolute 1e-7 holds what fp16 leaves of a weight: 2^-39 of (the largest probability x
+    the largest scale), so n 2^-36 of the largest scale for n tokens (2^3 > the largest level, its factor and the signs):
+    6e-8 of it, which the scales above 1 of these cases add here."""
+    import custom_ecc_cuda as ops
+    n, B = 4096, 1024
+    q, kp, vp, table = peaked(n, at, nats, v_scale, sink_v, g, rec, 64, seed=at + g)
+    o, tol, l, l_tol, _, _ = R.attend(q, kp, vp, table, [n])
+    top = R.fields(R.sequence(vp, table[0], 0, n))[2][:, 0].max()
+    tol = tol + n * 2.0 ** -36 * top
+    out, lse = ops.decode_attention_paged(cu(q).expand(B, g, 128).contiguous(), cu(kp), cu(vp), cu(table).expand(B, -1),
+                                          i32([n] * B), return_lse=True)
+    got = out.cpu().numpy().astype(np.float64).reshape(B, g, 128)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - o) <= tol).all(), np.max(np.abs(got - o) / tol)
+    assert (np.abs(lse.cpu().numpy() - l) <= l_tol).all()
+
+
 def test_decode_one_page_per_sequence_of_any_size():
     # a contiguous pool is a paged one with one page per sequence
     check_decode([100, 37, 0, 1], 8, 4, 100, 128, seed=3, width=1)
