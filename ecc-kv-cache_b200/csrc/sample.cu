@@ -15,9 +15,15 @@
 // One pass bins the tokens by their distance from the maximum, with counts and
 // masses; the bin in which top-k or top-p ends is then sorted on its own (a
 // bin of too many equal logits is descended by key bits, cluster_select.cuh);
-// a last pass draws.  Masses are sums of fixed-point numbers w * 2^S (S = 62 -
-// ceil(log2 V), at least 42 bits behind the point), so they do not depend on
-// the order of the additions, and atomics give the same bits every time.
+// a last pass draws.  Masses are sums of fixed-point numbers w * 2^S, so they do
+// not depend on the order of the additions, and atomics give the same bits every
+// time.  S leaves room for the row's own sum (62 - ceil(log2) of a bound of it:
+// of top-p from its counts, of a long top-k list from its entries, without a
+// filter from a pass of fp32 exponentials, 2 us for one row and 4 for 64): 41 to
+// 61 bits behind the point, and a running sum of V tokens is off by at most V
+// 2^-61 + 2^-45 of the whole, however long and flat the tail.  (With room for V
+// maxima in every row, 2^20 - 1 equal logits 14 below one peak were known to
+// 2^-23, and one draw in a hundred fell on a neighbour.)
 // A drawn token hangs on which side of a sum u * total falls: fp32 exponentials
 // would move one draw in a few thousand, so w is computed in fp64 to 2^-45
 // relative, by table and polynomial:
@@ -26,7 +32,7 @@
 // of the exponential function, 1989).
 //
 // Measured per call at 128256 bf16 logits: top-k 50 + top-p 0.9 17 us for one
-// row and 26 us for 64; top-p 0.9 alone 31 and 55 us; no filter 10 and 20 us;
+// row and 27 us for 64; top-p 0.9 alone 31 and 55 us; no filter 12 and 25 us;
 // greedy 4 and 7 us.  A row alone is bound by the latency of its phases (about
 // a microsecond per cluster barrier with the sums around it); 64 rows by the
 // issue of their passes, two CTAs a row: weights 10 us (45 instructions a token,
@@ -62,7 +68,6 @@ struct Args {
     int64_t *token;
     float *logprob;
     int slice;  // elements of a row per CTA
-    int S;      // fixed-point bits
 };
 
 template <class T>
@@ -110,6 +115,7 @@ struct Work {
     uint32_t best_at;
     float cta_best;       // of this CTA, read by the cluster
     uint32_t cta_best_at;
+    uint64_t bound[kMaxCluster];  // of the CTAs' masses, written by each of them
     uint32_t listed;      // entries of this CTA's list
     uint32_t kth, cut;    // written by rank 0
     uint64_t bin_mass;
@@ -128,29 +134,50 @@ struct Bins {
 };
 static_assert(sizeof(Bins) <= sizeof(Shared::hist), "room for the bins");
 
-// w * 2^S as an integer.  With y = (x - M) log2(e) / T, -62 < y <= 0, one product adds y to 192 + 2^-10, whose last
+// w * 2^S as an integer.  With y = (x - M) log2(e) / T, -63 < y <= 0, one product adds y to 192 + 2^-10, whose last
 // bit is 2^-45: the sum's bits are, from the top, floor(y') + 64 (y' = y + 2^-10), the first 9 bits behind the point
 // and the rest, from which 2^-10 is taken off again: |f| <= 2^-10.
 struct Mass {
     const double *tab;        // 2^(i / 512) 2^(S - 64)
     double best, scale;
-    float cut;                // what lies below has w < 2^-61: nothing of it is left by the rounding to 2^-S, S <= 51
+    float cut;                // what lies below has w < 2^-62.8: nothing of it is left by the rounding to 2^-S, S <= 61
     __device__ __forceinline__ Mass(const double *tab_, float best_, float temp) : tab(tab_), best(best_) {
         const double t = temp < INFINITY ? (double)temp : 1e300;
         scale = 1.442695040888963407 / t;
-        cut = __double2float_ru(best - 42.9 * t);  // finite: x = -inf lies below
+        cut = __double2float_ru(best - 43.6 * t);  // finite: x = -inf lies below
     }
     __device__ __forceinline__ uint64_t operator()(float x) const {  // the maximum itself: exactly 2^S
         const double d = (double)x - best, at = fma(d, scale, 192.0 + 1.0 / 1024.0);
-        const double y = x >= cut ? at : 130.0;  // (2^-62)
+        const double y = x >= cut ? at : 129.0;  // (2^-63)
         const int hi = __double2hiint(y);
         const double f = __hiloint2double((hi & 0xf) | 0x40600000, __double2loint(y)) - (128.0 + 1.0 / 1024.0);
         constexpr double c1 = 0.693147180559945309, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;  // 2^f = e^(f ln 2)
         const double p = fma(f, fma(f, fma(f, c3, c2), c1), 1.0);
         const double t = tab[(hi >> 4) & (kTab - 1)];
-        // the exponent of w by addition; adding 2^52 rounds the product to an integer
-        const double w = __hiloint2double(__double2hiint(t) + ((hi & 0xfe000) << 7), __double2loint(t));
-        return (uint64_t)__double_as_longlong(fma(p, w, 4503599627370496.0)) & 0xfffffffffffffull;
+        const double w = __hiloint2double(__double2hiint(t) + ((hi & 0xfe000) << 7), __double2loint(t));  // its exponent by addition
+        return __double2ull_rn(p * w);
+    }
+};
+
+// A bound of a row's mass, as a sum of integers, whatever the order: w in units of 2^-kBoundBits, to the nearest, in
+// the low bits of a float of exponent 23.  x - M, the scale and their product are off by 2^-24 of themselves, ex2 by
+// 2^-22: by less than 2^-16 of w where w reaches half a unit, and smaller ones are covered by a unit a token.
+constexpr int kBoundBits = 22;
+struct Bound {
+    float best, scale;
+    bool most;  // taken for n maxima: every weight is whole (T infinite), or the differences leave fp32's range
+    __device__ __forceinline__ Bound(float best_, float temp)
+        : best(best_), scale(fminf(1.44269504f / temp, 3e38f)), most(!(temp < INFINITY) || best > 1e31f) {}
+    __device__ __forceinline__ uint32_t operator()(float x) const {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(x - best, scale, (float)kBoundBits)));
+        return __float_as_uint(e + 8388608.0f) - 0x4b000000u;
+    }
+    // The fixed-point position S, 41 to 61, of n <= 2^20 tokens whose bounds add up to `sum`: their masses together stay
+    // below 2^62 (and half a unit each); unless `most`, 2^-S is less than 2^-61 of their sum and n 2^-21.
+    __device__ __forceinline__ int bits(uint64_t sum, int n) const {
+        const uint64_t all = most ? (uint64_t)n << kBoundBits : sum + (sum >> 15) + (uint64_t)n;
+        return min(61, 62 + kBoundBits - (64 - __clzll((long long)(all - 1))));  // 62 - ceil(log2(all 2^-22))
     }
 };
 
@@ -256,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     const Cluster cl;
     const int C = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int row = blockIdx.x / C;
-    for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab + (double)(a.S - 64));
+    for (int i = tid; i < kTab; i += kThreads) wk.tab[i] = exp2((double)i / kTab - 64.0);
     if (tid == 0) wk.listed = 0;
     pdl_trigger();
     pdl_wait();
@@ -344,7 +371,34 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
         best = 0.0f;
     }
     if (kCached) __syncthreads();  // the slice as the other threads read it from here on
+
+    // ---- masses: not before it is known how many bits S behind the point the sums leave room for
     const Mass mass(wk.tab, best, temp);
+    const Bound bound(best, temp);
+    const float mp = wk.set.min_p;
+    double unit = 0.0;   // 2^S
+    uint64_t least = 0;  // the smallest mass that min-p leaves
+    auto set_bits = [&](int S) {  // by the whole block
+        unit = __hiloint2double((1023 + S) << 20, 0);
+        for (int i = tid; i < kTab; i += kThreads) wk.tab[i] *= unit;
+        // w >= min_p as whole masses; the most likely token stays in any case
+        least = mp > 0.0f ? (uint64_t)ceil(fmin((double)mp, 1.0) * unit) : 0;
+        __syncthreads();
+    };
+    auto set_bits_by_a_pass = [&]() {
+        uint32_t sum = 0;   // of at most 128 tokens (V <= 2^20): 2^29
+        if (!bound.most) {  // cluster-uniform
+#pragma unroll 8
+            for (int i = tid; i < n; i += kThreads) sum += bound(load(i));
+        }
+        uint64_t all;
+        block_exclusive((uint64_t)sum, sh.warp64, &all);
+        if (tid < C) of_rank(cl, wk.bound, tid)[rank] = all;
+        cl.sync();
+        all = 0;
+        for (int r = 0; r < C; ++r) all += wk.bound[r];
+        set_bits(bound.bits(all, a.V));
+    };
 
     // What is kept so far: keys above `kth`, equal ones below the row position `cut`.
     uint32_t kth = 0, cut = 0xffffffffu;
@@ -354,9 +408,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     const int k = wk.set.top_k;
     const float p = wk.set.top_p;
     const bool by_count = k > 0 && k < a.V, by_mass = p < 1.0f;
-    const float mp = wk.set.min_p;
-    // w >= min_p as whole masses; the most likely token stays in any case
-    const uint64_t least = mp > 0.0f ? (uint64_t)ceil(fmin((double)mp, 1.0) * (double)(1ull << a.S)) : 0;
     const float u = wk.set.u;
     // cumulative mass > u * total, of whole masses: > floor(u * total); a number of 1 or more takes the last
     // kept token, one that is not above 0 the first
@@ -517,6 +568,15 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 gather(0, (int)at_k.slot, (uint32_t)(at_k.before + at_k.here));
                 if (rank != 0) return;  // nobody reads the other CTAs' shared memory any more
                 int kept = k;
+                if (k <= 256) {  // room for k maxima leaves S >= 54: k roundings are at most 2^-47 of the sum
+                    set_bits(min(61, 62 - (32 - __clz(k - 1))));
+                } else {
+                    uint32_t sum = 0;
+                    for (int i = tid; i < k; i += kThreads) sum += bound(key_value<T>((uint32_t)(list[i] >> 32)));
+                    uint64_t all;
+                    block_exclusive((uint64_t)sum, sh.warp64, &all);
+                    set_bits(bound.bits(all, k));
+                }
                 if (by_mass || least > 0) {
                     uint64_t sum = 0, want = 0, total;
                     if (by_mass) {
@@ -562,6 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 }
                 return;
             }
+            set_bits_by_a_pass();
         }
         if (by_mass && !by_count) {
             // ---- top-p alone: the bins' masses from counts and places tell where it ends, to 10^-4 of the mass;
@@ -575,10 +636,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
                 const float f = ((float)(uint32_t)wk.tot_mass[i] + 0.5f * n_b) * (1.0f / kPlaces);
                 constexpr float kChord = 0.015503561f;  // 1 - e^(-1/64)
                 const float m = expf(-(float)(rank * W + i) * (1.0f / 64.0f)) * (n_b * (1.0f - 1.52e-5f) - kChord * f);
-                wk.tot_mass[i] = (unsigned long long)((double)fmaxf(m, 0.0f) * (double)(1ull << a.S));
+                wk.tot_mass[i] = (unsigned long long)(fmaxf(m, 0.0f) * 1099511627776.0f);  // 2^40
             }
             __syncthreads();
             const uint64_t about = share_sums(sh.cross, cl, wk.tot_mass, sh.warp64);
+            // a bound too, with 1/8192 for its error; a bin is no closer than its token
+            set_bits(bound.bits((about >> (40 - kBoundBits)) + (about >> (53 - kBoundBits)), a.V));
             const uint64_t slack = about / 8192, aim = want_of(about);
             const uint64_t ends[2] = {aim > slack ? aim - slack : 1, min(aim + slack, about)};
             Crossing at[2];
@@ -720,6 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
     }
 
     // ---- the draw: masses of the warps' parts, then the part that holds the number
+    if (!by_count && !by_mass) set_bits_by_a_pass();
     auto kept_mass = [&](int i) -> uint64_t {
         const float x = load(i);
         if (!keep(value_key<T>(x), i)) return 0;
@@ -827,10 +891,6 @@ extern "C" int ecc_sample(const void *logits, int64_t row_stride, int dtype, int
     a.min_p0 = min_p_all;
     a.token = token;
     a.logprob = logprob;
-    int lg = 0;
-    while ((1ll << lg) < V) ++lg;
-    // the fixed-point value of one weight fits the 52 bits of the fp64 rounding, a row's sum 63 bits
-    a.S = std::min(51, 62 - lg);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     switch (dtype) {
         case ECC_SAMPLE_F16: return samp::launch<__half>(a, s);

@@ -1206,8 +1206,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
 
     Returns int64 [B]; with ``return_logprobs`` also fp32 [B], the log
     probability of each token among the kept ones.  NaN logits count as -inf; a
-    row without a logit above -inf gives -1 (log probability -inf).  The draw is
-    computed to 2^-45 of the probabilities and does not depend on timing."""
+    row without a logit above -inf gives -1 (log probability -inf).  Cumulative
+    probabilities are computed to V 2^-61 + 2^-45 and do not depend on timing."""
     _require_cuda(logits, "logits")
     if logits.dim() != 2 or logits.dtype not in _SAMPLE_TYPES or logits.shape[1] < 1:
         raise RuntimeError("logits must be float16, bfloat16 or float32 [B, V]")

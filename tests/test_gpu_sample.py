@@ -193,6 +193,61 @@ def test_sample_infinite_temperature_over_a_masked_row(V, allowed, dtype):
                 assert abs(float(lp[b]) + l) <= 2.0 ** -24 * l + 2.0 ** -40
 
 
+def exact_draws(x, u, p=1.0):
+    """Tokens of one row of logits for many numbers, at temperature 1: integer sums of weights to 2^-100, rounded from 60
+    decimal digits.  Also how far each number lies from the next border, as a part of the kept sum."""
+    from bisect import bisect_left, bisect_right
+    from decimal import Decimal, getcontext
+    from itertools import accumulate
+    getcontext().prec = 60
+    best = Decimal(float(x.max()))
+    weight = {v: int((Decimal(v) - best).exp() * (1 << 100)) for v in set(x.tolist())}
+    w = [weight[v] for v in x.tolist()]
+    ids = list(range(len(w)))
+    gap = 1.0
+    if p < 1:
+        order = sorted(ids, key=lambda i: (-x[i], i))
+        before = [0] + list(accumulate(w[i] for i in order))
+        m, shift = int(np.float64(np.float32(p)) * (1 << 60)), 60  # (exact: 24 bits)
+        border = -(-m * before[-1] >> shift)  # kept: what begins below p * total
+        c = bisect_left(before, border, 0, len(order))
+        gap = min(abs(b - border) for b in before[max(0, c - 1):c + 1]) / before[-1]
+        ids = sorted(order[:c])
+    cum = list(accumulate(w[i] for i in ids))
+    tok, gaps = [], []
+    for v in u.tolist():
+        target = int(np.float64(v) * (1 << 60)) * cum[-1] >> 60
+        j = bisect_right(cum, target)
+        tok.append(ids[j])
+        gaps.append(min(gap, min(abs(b - target) for b in cum[max(0, j - 1):j + 1]) / cum[-1]))
+    return np.array(tok), np.array(gaps)
+
+
+@pytest.mark.parametrize("dtype,V,low,high,p,B", [
+    ("bf16", 1 << 20, -13.875, -13.875, 1.0, 20000), ("bf16", 1 << 20, -15.0, -15.0, 1.0, 20000),
+    ("fp16", 1 << 20, -15.0, -13.0, 1.0, 20000), ("fp16", 128256, -11.75, -11.75, 1.0, 20000),
+    ("bf16", 128256, -20.0, -11.0, 1.0, 20000), ("bf16", 1 << 20, -13.875, -13.875, 0.75, 4000),
+    ("fp16", 128256, -12.0, -11.0, 0.9, 4000), ("fp32", 1 << 20, -14.0, -14.0, 1.0, 500),
+    ("fp16", 1 << 20, -40.0, -30.0, 1.0, 4000)])
+def test_sample_one_peak_and_a_long_flat_tail(dtype, V, low, high, p, B):
+    """Each token of the tail weighs next to nothing, all of them as much as the peak: a rounding of every weight in the
+    same direction would move the draws along the tail.  Running sums are off by at most V 2^-61 + 2^-45 of the whole
+    (each weight by half a unit 2^-S < 2^-61 of the sum, and by 2^-45 of itself), the same again for the total that
+    the number multiplies: draws that lie closer to a border are not compared, and there are few."""
+    import custom_ecc_cuda as ops
+    g = torch.Generator().manual_seed(V)
+    steps = int(round((high - low) * 8))
+    x = (low + torch.randint(0, steps + 1, (V,), generator=g) / 8.0).to(TYPES[dtype])
+    x[V // 3] = 0.0
+    u = torch.rand(B, generator=g)
+    tok, lp = ops.sample_tokens(x.cuda()[None].expand(B, V), u.cuda(), top_p=p, return_logprobs=True)
+    want, gaps = exact_draws(x.float().numpy(), u.numpy(), p)
+    clear = gaps > 2 * (V * 2.0 ** -61 + 2.0 ** -45)
+    assert clear.mean() > 0.999
+    assert np.array_equal(tok.cpu().numpy()[clear], want[clear]), (tok.cpu().numpy() != want)[clear].sum()
+    assert torch.isfinite(lp).all()
+
+
 def test_sample_distribution():
     """Evenly spaced numbers draw every token in proportion to its probability, to one part in their count."""
     import custom_ecc_cuda as ops
