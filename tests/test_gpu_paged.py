@@ -130,6 +130,15 @@ def test_decode_small_values_beside_a_dominating_token(at, nats, v_scale, sink_v
     assert (np.abs(lse.cpu().numpy() - l) <= l_tol).all()
 
 
+@pytest.mark.parametrize("lens,hq,rotate", [
+    ([16500] + [(0, 1, 33, 0, 70)[b % 5] for b in range(299)], 4, False),  # few slots a row: one group of threads joins 516
+    ([(0, 3, 0)[b % 3] for b in range(250)] + [9000, 7000] + [0] * 48, 2, True),
+    ([40003], 4, True), ([40003], 8, False)],  # 1251 partials, four groups
+    ids=["one long of 300", "two long of 300", "one of 40k", "one of 40k, group of 8"])
+def test_decode_joins_many_partials(lens, hq, rotate):
+    check_decode(lens, hq, 1, 64, 128, rotate=rotate, seed=len(lens) + hq)
+
+
 def test_decode_one_page_per_sequence_of_any_size():
     # a contiguous pool is a paged one with one page per sequence
     check_decode([100, 37, 0, 1], 8, 4, 100, 128, seed=3, width=1)
