@@ -432,8 +432,8 @@ __device__ __forceinline__ void sort_descending(unsigned long long *x, int n) {
     __syncthreads();
 }
 
-// Launch with a cluster of `c` CTAs per row (y), as a dependent of the kernel
-// before it on the stream.
+// Launch with a cluster of `c` neighbouring CTAs per row, as a dependent of the
+// kernel before it on the stream.
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_cluster(void (*kernel)(KArgs...), int c, int64_t rows, size_t smem, cudaStream_t s,
                                          Args &&...args) {

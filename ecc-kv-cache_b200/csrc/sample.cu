@@ -12,10 +12,17 @@
 //   A row without a logit above -inf: token -1, logprob -inf.
 //
 // No sort of the row: one cluster of CTAs per row keeps it in shared memory.
-// One pass bins the tokens by their distance from the maximum, with counts and
-// masses; the bin in which top-k or top-p ends is then sorted on its own (a
-// bin of too many equal logits is descended by key bits, cluster_select.cuh);
-// a last pass draws.  Masses are sums of fixed-point numbers w * 2^S, so they do
+// A pass bins the tokens by their distance from the maximum:
+//   top-k: counts alone.  When everything down to the bin of the k-th fits the
+//     list (4096), one CTA sorts that and finishes, top-p and min-p included.
+//   top-p alone: counts and places inside the bins, from which each bin's mass
+//     is estimated; a second pass adds up the exact masses above the bins around
+//     the estimated end and lists theirs, and the draw takes its sums over.
+//   otherwise (a long top-k list with top-p; an end that the estimate missed):
+//     counts and exact masses, and the bin in which the set ends is sorted on its
+//     own.  A bin of too many (nearly) equal logits is descended by key bits
+//     (cluster_select.cuh).
+// Then a pass draws.  Masses are sums of fixed-point numbers w * 2^S, so they do
 // not depend on the order of the additions, and atomics give the same bits every
 // time.  S leaves room for the row's own sum (62 - ceil(log2) of a bound of it:
 // of top-p from its counts, of a long top-k list from its entries, without a
@@ -648,7 +655,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             crossings(sh.cross, cl, wk.tot_mass, ends, at, sh.warp64);
             const int b0 = (int)at[0].slot, b1 = ends[1] < about ? (int)at[1].slot : kBins - 1;
             {
-                const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : 3e38f;  // (what lies further off has no mass)
+                const float d0 = (float)b0, d1 = b1 < kBins - 1 ? (float)(b1 + 1) : 3e38f;
+                // (mass beyond d1, at a vast temperature: the list misses the end, and the exact search below finds it)
                 int lo, hi;
                 warp_part(n, lo, hi);
                 uint64_t all = 0, above = 0, part = 0;
