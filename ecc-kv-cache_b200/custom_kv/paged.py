@@ -336,6 +336,20 @@ class PagedErrorCorrectedCache(_HFCache):
             query_length = int(query_length.shape[0]) if query_length.dim() > 0 else int(query_length)
         return (self.get_seq_length(layer_idx) + int(query_length), 0)
 
+    # What transformers' Cache does to its own layers, which this cache has none of: beams, candidates that are taken
+    # back and batches that change are refused, not passed over.
+    def crop(self, max_length: int) -> None:
+        raise RuntimeError("PagedErrorCorrectedCache cannot be cropped (release() ends a sequence, evict() cuts it)")
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        raise RuntimeError("PagedErrorCorrectedCache cannot be reordered: no beam search")
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        raise RuntimeError("PagedErrorCorrectedCache has a fixed number of slots")
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        raise RuntimeError("PagedErrorCorrectedCache has a fixed number of slots (release() ends a sequence)")
+
     @property
     def is_compileable(self) -> bool:
         return False

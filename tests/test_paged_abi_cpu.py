@@ -161,6 +161,17 @@ def test_paged_cache_refuses_cpu_device():
         PagedErrorCorrectedCache(cfg, device="cpu")
 
 
+@pytest.mark.parametrize("call,arg", [("crop", 3), ("reorder_cache", torch.tensor([1, 0])), ("batch_repeat_interleave", 2),
+                                      ("batch_select_indices", torch.tensor([1]))])
+def test_paged_cache_refuses_what_it_cannot_do(call, arg):
+    """transformers' Cache does these to its layers; this cache has none, so they would pass without doing anything."""
+    from custom_kv import PagedErrorCorrectedCache
+    cache = object.__new__(PagedErrorCorrectedCache)
+    cache.layers = []
+    with pytest.raises(RuntimeError, match="PagedErrorCorrectedCache"):
+        getattr(cache, call)(arg)
+
+
 def test_written_weights_must_not_overlap():
     import custom_ecc_cuda as ops
     cpu = torch.device("cpu")
