@@ -24,8 +24,8 @@
 // Measured at 8 sequences x 65531 tokens, 32 query and 8 kv heads, pages of 128
 // tokens (1.07 GB of blocks): 229 us with the merge, 4.7 TB/s; the loads alone
 // take 169 us.  It is bound by the latency of dependent instructions at three
-// warps of 168 registers per scheduler (ncu: issue 56 %, shared-memory
-// wavefronts 60 %, ALU 50 %, tensor 36 %), and in runs of seconds by the 1000 W
+// warps of 168 registers per scheduler (ncu: issue 57 %, L1 62 %,
+// ALU 52 %, tensor 37 %), and in runs of seconds by the 1000 W
 // power cap.
 #include <algorithm>
 

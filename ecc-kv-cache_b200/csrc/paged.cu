@@ -36,7 +36,7 @@ namespace paged {
 // fp16 written), where filling the output with zeros alone takes 44 us.  A
 // butterfly kernel with four lanes per vector (72 warp instructions and 21 L1
 // wavefronts a vector, against 47 and 12) took 63 us, bound by L1; without the
-// volatile order, 57 to 67 us.
+// volatile order, 57 to 67 us.  In the stored basis (kRotate false) 53 us too.
 constexpr int kReadWarps = 8;
 constexpr int kReadVecs = 16;                       // per warp and step
 constexpr int kReadTile = kReadWarps * kReadVecs;   // per CTA and step
