@@ -286,7 +286,7 @@ decode_paged_kernel(const __grid_constant__ CUtensorMap mkc, const __grid_consta
     Lane<G, true> L;
     L.g = lane >> 2;
     L.c = lane & 3;
-    L.scale_log2_0 = a.scale_log2;
+    L.scale_log2 = a.scale_log2;
     // query words of lane (g, c): dims 32c.. of query head g of the group (as in decode_tma_kernel)
     auto load_q = [&](uint4 (&qw)[4], int b, int h) {
         const int qh = (G <= 4) ? (L.g & 3) : L.g;

@@ -235,7 +235,7 @@ __device__ __forceinline__ uint2 lut_entry(const uint32_t *cent, int v, int lane
 __device__ __forceinline__ uint32_t e5m2_pair(uint32_t w, int j) { return __byte_perm(w, 0u, j ? 0x3424u : 0x1404u); }
 
 // Consumer lane state for one work item.  kFine: the paired table above, and
-// a query that is scaled to a largest magnitude in [1, 2) and, when it is
+// a query that is scaled, head by head, to a largest magnitude in [1, 2) and, when it is
 // rotated here, not rounded to fp16 but carried as fp16 plus remainder (for
 // groups of up to 4 heads in the idle columns 4..7 of the QK operand,
 // otherwise as e5m2 words).  For groups of at most 4 query heads
@@ -250,7 +250,7 @@ struct Lane {
     uint32_t qc[8][2];
     uint32_t ql[kLoWords ? 8 : 1];  // remainders of the four values of qc[m], e5m2
     uint32_t qs[8][2];  // q of the sign products, k slot of bit p scaled by 2^-(ssh + kexp(p))
-    float sgn2;         // 2^(ssh + 1): q.s = sgn2 * (sign product) - sum(q)
+    float sgn2;         // 2^(ssh + 1): q.s = sgn2 * (sign product) - sum(q); kFine: 2
     float qsum[2];
     // PV accumulators: o[i] rows g / g+8 = dims 16g + 2i / 16g + 2i + 1 (code
     // byte i of the lane's 8 V code bytes), columns = the n8 operand columns
@@ -260,8 +260,8 @@ struct Lane {
     uint32_t voff;  // this lane's byte offset in the swizzled V code box (see load_v)
     uint32_t soff;  // this lane's byte offset in the swizzled syndrome boxes (see qk, load_v)
     int g, c;
-    float scale_log2;   // of the scores, with the query's scaling
-    float scale_log2_0;  // kFine: without it
+    float scale_log2;   // of the scores; kFine: without the query's scaling
+    float scale_up[2];  // kFine: with it, of heads 2c, 2c + 1
     uint32_t lane8, lane_hi;  // kFine: offsets in the paired table
     int vexp;  // kFine: exponent field of the largest V scale or 2 alpha so far, 1..31 (see tile)
     __device__ __forceinline__ float v_up() const { return kFine ? __int_as_float((127 + 29 - vexp) << 23) : 1.0f; }
@@ -310,14 +310,15 @@ struct Lane {
             }
         }
         if constexpr (kFine) {
-            float qmax = 0.0f;
+            float qmax = 0.0f;  // of the lane's head: the heads of a group may differ by any factor
 #pragma unroll
             for (int k = 0; k < 32; ++k) qmax = fmaxf(qmax, fabsf(x[k]));
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, off));
+            for (int off = 1; off < 4; off <<= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, off));
             const int e2 = qmax > 0.0f ? max(-100, min(100, ((__float_as_int(qmax) >> 23) & 0xff) - 127)) : 0;
-            const float down = __int_as_float((127 - e2) << 23);
-            scale_log2 = scale_log2_0 * __int_as_float((127 + e2) << 23);
+            const float down = __int_as_float((127 - e2) << 23), up = scale_log2 * __int_as_float((127 + e2) << 23);
+            scale_up[0] = __shfl_sync(0xffffffffu, up, 4 * (2 * c));
+            scale_up[1] = __shfl_sync(0xffffffffu, up, 4 * (2 * c + 1));
 #pragma unroll
             for (int k = 0; k < 32; ++k) x[k] *= down;
         }
@@ -335,16 +336,19 @@ struct Lane {
         }
         // sign-product operand: scale 2^-ssh keeps q * 2^(14 - ssh) < 2^15
         // for the largest |q| of the group (q is fp16, the scalings are
-        // exact powers of two)
+        // exact powers of two); kFine: |q| <= 2, so ssh = 0
         {
-            float qmax = 0.0f;
+            int ssh = 0;
+            if constexpr (!kFine) {
+                float qmax = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) qmax = fmaxf(qmax, fabsf(x[k]));
+                for (int k = 0; k < 32; ++k) qmax = fmaxf(qmax, fabsf(x[k]));
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, off));
-            const int e2 = (qmax > 0.0f) ? ((__float_as_int(qmax) >> 23) & 0xff) - 127 : 0;
-            const int ssh = max(0, e2);
-            sgn2 = __int_as_float((ssh + 1 + 127) << 23);
+                for (int off = 1; off < 32; off <<= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, off));
+                const int e2 = (qmax > 0.0f) ? ((__float_as_int(qmax) >> 23) & 0xff) - 127 : 0;
+                ssh = max(0, e2);
+                sgn2 = __int_as_float((ssh + 1 + 127) << 23);
+            }
             if constexpr (kLoWords) {
                 // a remainder is at most 2^-11; an e5m2 keeps three bits of it down to 2^-14 and steps of 2^-16
                 // below, so at most 2^-14 of the fp16 rounding's 2^-11 is left
@@ -457,7 +461,7 @@ struct Lane {
         constexpr float kUnit = kFine ? 1.0f / kCentScale : 1.0f;  // of the table's centroids
         const float k_sa = h_lo(kma.x) * kUnit, k_za = h_hi(kma.x), k_aa = h_lo(kma.y);
         const float k_sb = h_lo(kmb.x) * kUnit, k_zb = h_hi(kmb.x), k_ab = h_lo(kmb.y);
-        const float k_ga = k_aa * sgn2, k_gb = k_ab * sgn2, k_da = k_za - k_aa, k_db = k_zb - k_ab;
+        const float sgn = kFine ? 2.0f : sgn2, k_ga = k_aa * sgn, k_gb = k_ab * sgn, k_da = k_za - k_aa, k_db = k_zb - k_ab;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float xa = fmaf(k_sa, sc[e], fmaf(k_ga, ss[e], k_da * qsum[e]));
@@ -466,8 +470,9 @@ struct Lane {
                 xa += __shfl_xor_sync(0xffffffffu, xa, 2);
                 xb += __shfl_xor_sync(0xffffffffu, xb, 2);
             }
-            s2[e] = va ? xa * scale_log2 : -INFINITY;
-            s2[2 + e] = vb8 ? xb * scale_log2 : -INFINITY;
+            const float sl = kFine ? scale_up[e] : scale_log2;
+            s2[e] = va ? xa * sl : -INFINITY;
+            s2[2 + e] = vb8 ? xb * sl : -INFINITY;
         }
     }
 

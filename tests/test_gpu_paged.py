@@ -130,6 +130,27 @@ def test_decode_small_values_beside_a_dominating_token(at, nats, v_scale, sink_v
     assert (np.abs(lse.cpu().numpy() - l) <= l_tol).all()
 
 
+@pytest.mark.parametrize("g", [2, 4, 8])
+@pytest.mark.parametrize("ratio,k_scale", [(1e-2, 50), (1e-3, 500), (1e-4, 5000), (1e-5, 5000), (3000.0, 0.01)])
+def test_decode_heads_of_unlike_magnitude(g, ratio, k_scale):
+    """One head of a group is 1 / ratio times the others: each keeps the precision of its own magnitude."""
+    import custom_ecc_cuda as ops
+    rng = np.random.default_rng(g)
+    kp, vp, table = R.make_pools([300], 64, 1, 128, rng)
+    for t in range(300):
+        meta = kp[table[0, t // 64], 0, t % 64, 80:86].view(np.float16)
+        meta[:] = (meta.astype(np.float64) * k_scale).astype(np.float16)
+    q = rng.normal(size=(1, g, 128))
+    q[:, 1:] *= ratio
+    q = q.astype(np.float16)
+    for rotate in (False, True):
+        o, tol, l, l_tol, _, _ = R.attend(q, kp, vp, table, [300], rotate=rotate)
+        out, lse = ops.decode_attention_paged(cu(q), cu(kp), cu(vp), cu(table), i32([300]), rotate_q=rotate,
+                                              unrotate_out=rotate, return_lse=True)
+        assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(1, g, 128) - o) <= tol).all()
+        assert (np.abs(lse.cpu().numpy() - l) <= l_tol).all(), np.max(np.abs(lse.cpu().numpy() - l) / l_tol)
+
+
 @pytest.mark.parametrize("lens,hq,rotate", [
     ([16500] + [(0, 1, 33, 0, 70)[b % 5] for b in range(299)], 4, False),  # few slots a row: one group of threads joins 516
     ([(0, 3, 0)[b % 3] for b in range(250)] + [9000, 7000] + [0] * 48, 2, True),
