@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_consta
             }
             __syncthreads();
             const uint64_t about = share_sums(sh.cross, cl, wk.tot_mass, sh.warp64);
-            // a bound too, with 1/8192 for its error; a bin is no closer than its token
+            // with 1/8192 for its error, a bound of the row's mass too (the last bin counts at its near edge)
             set_bits(bound.bits((about >> (40 - kBoundBits)) + (about >> (53 - kBoundBits)), a.V));
             const uint64_t slack = about / 8192, aim = want_of(about);
             const uint64_t ends[2] = {aim > slack ? aim - slack : 1, min(aim + slack, about)};
